@@ -77,7 +77,7 @@ enum ns_act_mode {
 /* Bits of the per-device error word. */
 #define NS_DEVERR_GRID_WAIT 1u  /* grid-wide barrier ran out */
 #define NS_DEVERR_COPY_WAIT 2u  /* bulk-copy completion wait ran out */
-#define NS_DEVERR_ROUTE 4u      /* an invalid expert id, token id or position */
+#define NS_DEVERR_ROUTE 4u      /* an invalid expert id, token id, position or tree */
 
 const char* ns_last_error(void);
 int ns_abi_version(void);
@@ -367,6 +367,162 @@ int ns_attn_block(const ns_attn_block_t* p, void* workspace, size_t workspace_by
  */
 int ns_embed(const void* table, int dtype, int64_t rows, int H, const int32_t* token, float* out,
              ns_stream_t stream);
+
+/*
+ * Speculative decoding: several drafted tokens per sequence and step, as a tree
+ * over each sequence's cached context.  No reference counterpart: the reference
+ * decodes one token at a time (neurostream/model/gpt_oss.py:207-228); rotary
+ * positions, the cache layout, sinks and sliding windows follow its operators.
+ *
+ * A call covers B sequences of T nodes each.  lens[b] is the sequence's context:
+ * cache slots [0, lens[b]) hold its keys and values, and node t of the step uses
+ * slot lens[b] + t.  parents[b * T + t] < t is the node it continues, -1 hangs it on
+ * the context itself and -2 marks an unused node; parents = NULL is a chain (node
+ * t continues node t - 1).  depth(t) counts a node's ancestors; its position is
+ * lens[b] + depth(t).  lens and parents are read on the device, so one captured
+ * graph serves every context and tree.  A bad length, parent or slot raises
+ * NS_DEVERR_ROUTE; its node counts as unused, and nothing is read or written out
+ * of bounds.
+ */
+#define NS_TREE_MAX_NODES 64   /* nodes per sequence when parents are given, and of ns_tree_attn */
+
+/*
+ * Rotary positions of new tokens and their append to the cache, in one launch:
+ * the first rotary_dim dims of q and k are rotated by the table row of their
+ * position (pairs (i, i + rotary_dim/2), or (2i, 2i + 1) when interleaved; the
+ * rest is passed through), q is written to q_out and k, v to their cache slots.
+ * Generalises neurostream/compute/ops.py:136-151 `apply_rope` and
+ * neurostream/model/qwen3.py:74-85 `KVCache.append` to batches, trees, partial
+ * and interleaved rotation and 16-bit caches.
+ * Tables: fp32, n_pos rows of at least rotary_dim/2 columns, row stride
+ * table_stride.  positions (B x T int32) replaces lens + depth as the table row
+ * when given.  q, k or v may be NULL (nothing is done for it); q_out may be q.
+ * Rows of unused nodes: q_out is zero, the cache is left alone.  Any T when
+ * parents is NULL, else at most NS_TREE_MAX_NODES.  Strides are in elements, the
+ * innermost dimension is contiguous.  fp32 arithmetic, one rounding at the end.
+ */
+typedef struct ns_rope_append {
+  int B, T, n_head, n_head_kv, head_dim, rotary_dim;
+  int interleaved;
+  int dtype;                  /* q, k, v, q_out */
+  int cache_dtype;            /* k_cache, v_cache */
+  int n_pos;                  /* rows of the tables */
+  int max_ctx;                /* slots each cache holds */
+  const int32_t* lens;        /* B */
+  const int32_t* parents;     /* B x T, or NULL: a chain */
+  const int32_t* positions;   /* B x T, or NULL */
+  const float* rope_cos;
+  const float* rope_sin;
+  int64_t table_stride;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  int64_t q_stride[3];        /* sequence, token, head */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t qo_stride[3];
+  int64_t kc_stride[3];       /* sequence, head, slot */
+  int64_t vc_stride[3];
+} ns_rope_append_t;
+int ns_rope_append(const ns_rope_append_t* p, ns_stream_t stream);
+
+/*
+ * Attention of every node of the step over the cache: a node sees its sequence's
+ * context (slots below lens[b]), its ancestors and itself; with window > 0 only
+ * positions above its own minus window.  sinks (n_head fp32, or NULL) adds one
+ * logit per head to the softmax, as neurostream/model/gpt_oss.py:73-87
+ * `sink_attention`.  T = 1 is plain decode.  Keys and values of the nodes are in
+ * the cache already (ns_rope_append).  out rows of unused nodes, and of nodes
+ * that see nothing, are zero; what no node may see is not used, whatever it holds.
+ * q, caches and out have one type: fp32 (products at fp32 precision), fp16 or
+ * bf16 (fp32 softmax; probabilities rounded to the type for the product with
+ * the values).  head_dim up to 128, a multiple of 8; any number of query heads per kv head.
+ * Caches: 16-byte aligned, their strides multiples of 16 bytes.
+ * Workspace: ns_tree_attn_workspace_bytes, 256-byte aligned, no initialisation.
+ */
+typedef struct ns_tree_attn {
+  int B, T, n_head, n_head_kv, head_dim;
+  int max_ctx;                /* slots each cache holds */
+  int window;                 /* 0: all of the context */
+  int dtype;
+  float scale;                /* 1 / sqrt(head_dim) */
+  const int32_t* lens;        /* B */
+  const int32_t* parents;     /* B x T, or NULL: a chain */
+  const float* sinks;         /* n_head fp32, or NULL */
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* out;
+  int64_t q_stride[3];        /* sequence, token, head */
+  int64_t o_stride[3];
+  int64_t kc_stride[3];       /* sequence, head, slot */
+  int64_t vc_stride[3];
+} ns_tree_attn_t;
+int ns_tree_attn_workspace_bytes(const ns_tree_attn_t* p, size_t* bytes);
+int ns_tree_attn(const ns_tree_attn_t* p, void* workspace, size_t workspace_bytes, ns_stream_t stream);
+
+/*
+ * Verification of a drafted tree against the target's logits from given random
+ * numbers.  Node 0 is the last accepted token (its parent is -1); tokens[b, t] is
+ * node t's token and logits[b, t] the target's logits after it.  The walk starts at
+ * node 0.  At node n, with r = softmax(logits[n] / temperature) and q the
+ * distribution its children were drawn from without replacement
+ * (draft_probs[b, n]; NULL: every child for certain), children in node order:
+ *   accept c if uniforms[c] * q(c) < r(c) and go on from c; otherwise
+ *   r = normalise(max(r - q, 0)) (kept if nothing is left), q(c) = 0, q renormalised.
+ * When no child is accepted, the next token is drawn from r: the index with the
+ * largest r(x) / race[x], race holding draws of Exp(1).  The tokens emitted this
+ * way are distributed as the target's own.  temperature[b] = 0: r is all on the
+ * largest logit (lowest index on ties), a child is accepted if it is that token,
+ * and it is the next token.  A NaN logit counts as -inf, +inf as the largest
+ * finite number; a row of nothing else than -inf accepts nothing and gives token -1.
+ * Results: path (B x T: accepted nodes from node 0 on, then -1), n_accepted (B:
+ * accepted nodes, node 0 not counted), next_token (B).
+ */
+typedef struct ns_tree_verify {
+  int B, T, V;
+  int dtype;                  /* of logits */
+  int draft_dtype;            /* of draft_probs */
+  const int32_t* tokens;      /* B x T */
+  const int32_t* parents;     /* B x T, or NULL: a chain */
+  const void* logits;         /* B x T x V */
+  const void* draft_probs;    /* B x T x V, or NULL */
+  const float* uniforms;      /* B x T, in [0, 1) */
+  const float* race;          /* B x V, positive */
+  const float* temperature;   /* B, or NULL: 1 */
+  int64_t l_stride[2];        /* logits: sequence, node */
+  int64_t d_stride[2];        /* draft_probs: sequence, node */
+  int32_t* path;              /* B x T */
+  int32_t* n_accepted;        /* B */
+  int32_t* next_token;        /* B */
+} ns_tree_verify_t;
+int ns_tree_verify(const ns_tree_verify_t* p, ns_stream_t stream);
+
+/*
+ * Moves the accepted path's keys and values into place after a verified step:
+ * slot lens[b] + path[b, i] -> lens[b] + i for 0 <= i <= n_accepted[b], in every
+ * layer's two caches, one launch; new_lens[b] = lens[b] + 1 + n_accepted[b].
+ * path rows ascend strictly (path[i] >= i); n_accepted = -1 moves nothing.  The
+ * caches share one layout (strides, type).  new_lens must not be lens.
+ */
+#define NS_COMMIT_MAX_LAYERS 128
+typedef struct ns_path_commit {
+  int n_layer, B, T, n_head_kv, head_dim;
+  int max_ctx;
+  int dtype;
+  const int32_t* lens;        /* B */
+  const int32_t* path;        /* B x T */
+  const int32_t* n_accepted;  /* B */
+  int32_t* new_lens;          /* B */
+  int64_t kc_stride[3];       /* sequence, head, slot */
+  int64_t vc_stride[3];
+  void* k_cache[NS_COMMIT_MAX_LAYERS];
+  void* v_cache[NS_COMMIT_MAX_LAYERS];
+} ns_path_commit_t;
+int ns_path_commit(const ns_path_commit_t* p, ns_stream_t stream);
 
 /*
  * Sum of n fp32 values over the `world` ranks of one node (one process per

@@ -8,6 +8,7 @@ a C ABI (include/ns_b200.h), with Python mirrors of the reference's operators on
 * ``nurostream_b200.fused``   -- can_fuse / fused_gemv / dequantize
 * ``nurostream_b200.moe``     -- route, MoeLayer, the GPT-OSS / Qwen3 MoE drop-ins
 * ``nurostream_b200.gptoss``  -- GptOssDecoder: a whole decode token in one CUDA graph
+* ``nurostream_b200.spec``    -- speculative decoding: rope_append, tree_attention, verify_tree, commit_path
 * ``nurostream_b200.install`` -- patch an importable reference package in place
 
 Importing the package loads no native code; the library is loaded on first use.

@@ -113,6 +113,50 @@ class PeerReduceParams(C.Structure):
                 ("slots", C.c_void_p * NS_MAX_PEERS), ("ctr", C.c_void_p)]
 
 
+NS_TREE_MAX_NODES, NS_COMMIT_MAX_LAYERS = 64, 128
+_S2, _S3 = C.c_int64 * 2, C.c_int64 * 3
+
+
+class RopeAppendParams(C.Structure):
+    """Mirror of ns_rope_append_t."""
+
+    _fields_ = [("B", C.c_int), ("T", C.c_int), ("n_head", C.c_int), ("n_head_kv", C.c_int), ("head_dim", C.c_int),
+                ("rotary_dim", C.c_int), ("interleaved", C.c_int), ("dtype", C.c_int), ("cache_dtype", C.c_int),
+                ("n_pos", C.c_int), ("max_ctx", C.c_int), ("lens", C.c_void_p), ("parents", C.c_void_p),
+                ("positions", C.c_void_p), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
+                ("table_stride", C.c_int64), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("q_out", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("q_stride", _S3),
+                ("k_stride", _S3), ("v_stride", _S3), ("qo_stride", _S3), ("kc_stride", _S3), ("vc_stride", _S3)]
+
+
+class TreeAttnParams(C.Structure):
+    """Mirror of ns_tree_attn_t."""
+
+    _fields_ = [("B", C.c_int), ("T", C.c_int), ("n_head", C.c_int), ("n_head_kv", C.c_int), ("head_dim", C.c_int),
+                ("max_ctx", C.c_int), ("window", C.c_int), ("dtype", C.c_int), ("scale", C.c_float),
+                ("lens", C.c_void_p), ("parents", C.c_void_p), ("sinks", C.c_void_p), ("q", C.c_void_p),
+                ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("out", C.c_void_p), ("q_stride", _S3),
+                ("o_stride", _S3), ("kc_stride", _S3), ("vc_stride", _S3)]
+
+
+class TreeVerifyParams(C.Structure):
+    """Mirror of ns_tree_verify_t."""
+
+    _fields_ = [("B", C.c_int), ("T", C.c_int), ("V", C.c_int), ("dtype", C.c_int), ("draft_dtype", C.c_int),
+                ("tokens", C.c_void_p), ("parents", C.c_void_p), ("logits", C.c_void_p), ("draft_probs", C.c_void_p),
+                ("uniforms", C.c_void_p), ("race", C.c_void_p), ("temperature", C.c_void_p), ("l_stride", _S2),
+                ("d_stride", _S2), ("path", C.c_void_p), ("n_accepted", C.c_void_p), ("next_token", C.c_void_p)]
+
+
+class PathCommitParams(C.Structure):
+    """Mirror of ns_path_commit_t."""
+
+    _fields_ = [("n_layer", C.c_int), ("B", C.c_int), ("T", C.c_int), ("n_head_kv", C.c_int), ("head_dim", C.c_int),
+                ("max_ctx", C.c_int), ("dtype", C.c_int), ("lens", C.c_void_p), ("path", C.c_void_p),
+                ("n_accepted", C.c_void_p), ("new_lens", C.c_void_p), ("kc_stride", _S3), ("vc_stride", _S3),
+                ("k_cache", C.c_void_p * NS_COMMIT_MAX_LAYERS), ("v_cache", C.c_void_p * NS_COMMIT_MAX_LAYERS)]
+
+
 _P, _I, _I64, _U64, _SZ, _F = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_size_t, C.c_float
 
 SIGNATURES = {
@@ -143,6 +187,11 @@ SIGNATURES = {
     "ns_attn_decode": (_I, [C.POINTER(AttnDecodeParams), _P, _SZ, _P]),
     "ns_embed": (_I, [_P, _I, _I64, _I, _P, _P, _P]),
     "ns_attn_block_workspace_bytes": (_I, [C.POINTER(AttnBlockParams), C.POINTER(_SZ)]),
+    "ns_rope_append": (_I, [C.POINTER(RopeAppendParams), _P]),
+    "ns_tree_attn_workspace_bytes": (_I, [C.POINTER(TreeAttnParams), C.POINTER(_SZ)]),
+    "ns_tree_attn": (_I, [C.POINTER(TreeAttnParams), _P, _SZ, _P]),
+    "ns_tree_verify": (_I, [C.POINTER(TreeVerifyParams), _P]),
+    "ns_path_commit": (_I, [C.POINTER(PathCommitParams), _P]),
     "ns_attn_block": (_I, [C.POINTER(AttnBlockParams), _P, _SZ, _P]),
 }
 

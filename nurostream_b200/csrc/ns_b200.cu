@@ -11,3 +11,7 @@
 #include "attn_block.cu"
 #include "synth.cu"
 #include "peer.cu"
+#include "rope.cu"
+#include "tree_attn.cu"
+#include "verify.cu"
+#include "commit.cu"

@@ -1,0 +1,776 @@
+// ns_tree_attn: attention of every node of a drafted tree over its sequence's cache.
+//
+// Generalises the core of neurostream/model/gpt_oss.py:73-114 (sink_attention over a KV cache, with the
+// sliding window) from one token to B sequences of T nodes:
+//   out[t] = sum_j p_j v_j / (sum_j p_j + e^(sink - m)),  p_j = e^(s_j - m),  s_j = scale q_t . k_j
+// over the keys j that node t sees: the context below lens[b] (within the window) and its ancestors.
+//
+// The rep query heads of a kv head and the T nodes are the rows of one matrix (rows = T * rep), so the
+// keys and values of a kv head are read once for all of them.  An item is (sequence, kv head, tile of
+// rows); its keys are walked in blocks with a running maximum and sum.  Contexts differ, are known on
+// the device alone and are long, so the blocks of all items are one list, cut into equal runs, one per
+// CTA: every SM gets the same work whatever the lengths are.  A run that covers an item writes the
+// result; an item cut between CTAs leaves partial (maximum, sum, output) rows in the workspace, and a
+// second kernel joins them in order of the keys (results do not depend on timing).
+//
+// Within a CTA eight warps are WM groups of 16 rows by WK = 8 / WM groups of keys, so that a single
+// row's 16-row tile still keeps eight warps on the stream; the key groups join through shared memory.
+// Blocks arrive by cp.async in a ring of three stages.  16-bit products are mma.m16n8k16; fp32
+// products split each operand into two tf32 parts and add three mma.m16n8k8 (the product of the two
+// low parts, 2^-22 of the whole, is dropped), and the sum over a block joins the running output in
+// plain fp32 additions.
+#include "tree.cuh"
+
+namespace ns {
+
+constexpr int kTaWarps = 8;
+constexpr int kTaThreads = kTaWarps * 32;
+constexpr int kTaStages = 3;
+
+template <int DT, int HD>
+struct TaCfg {
+  static constexpr int kEl = DT == NS_F32 ? 4 : 2;       // bytes per element
+  static constexpr int kBlock = DT == NS_F32 ? 64 : 128;  // keys per block
+  static constexpr int kRowBytes = HD * kEl;
+  static constexpr int kTile = kBlock * kRowBytes;        // bytes of a key (or value) block
+  static constexpr int kSmem = kTaStages * 2 * kTile;
+};
+
+struct TaArgs {
+  ns_tree_attn_t p;
+  int rep;         // query heads per kv head
+  int row_tiles;   // tiles of rows of one (sequence, kv head)
+  int grid;        // runs, at most: none is empty (ta_runs)
+  float* part_o;   // [2 * grid][rows per tile][HD]
+  float* part_ml;  // [2 * grid][rows per tile][2]
+};
+
+struct TaShared {
+  uint64_t anc[kTreeMax];   // of the sequence at hand
+  int depth[kTreeMax];
+  int max_depth, bad_lo, bad_hi;
+  uint32_t bad_keys[4];     // keys of the block whose values are not finite and not seen by all
+  float wm[kTaWarps][16], wl[kTaWarps][16];
+};
+
+// Keys [lo, hi) of sequence b that any node may see, and how many blocks they are.
+struct TaSpan {
+  int lo, hi, len;
+};
+__device__ __forceinline__ TaSpan ta_span(const ns_tree_attn_t& p, int b) {
+  const int n = tree_len(p.lens, b, p.max_ctx);
+  if (n < 0) return TaSpan{0, 0, 0};
+  const int lo = p.window > 0 ? max(0, n - p.window + 1) : 0;
+  return TaSpan{lo, min(n + p.T, p.max_ctx), n};
+}
+
+// Position in the list of all blocks: sequences in order, then kv heads, row tiles, blocks of keys.
+struct TaPos {
+  int b, h, rt, blk, nblk;
+};
+
+// Runs of a list of `total` blocks, and the first block of run i.
+__device__ __forceinline__ int ta_runs(const TaArgs& a, int64_t total) { return (int)(total < a.grid ? total : a.grid); }
+__device__ __forceinline__ int64_t ta_first_unit(int64_t total, int runs, int i) { return total * i / runs; }
+
+// The sequence and offset of unit u, by a walk over the sequences (all threads alike).
+template <int BN>
+__device__ __forceinline__ int64_t ta_total(const TaArgs& a) {
+  int64_t n = 0;
+  for (int b = 0; b < a.p.B; ++b) {
+    const TaSpan s = ta_span(a.p, b);
+    n += (int64_t)((s.hi - s.lo + BN - 1) / BN);
+  }
+  return n * a.p.n_head_kv * a.row_tiles;
+}
+
+template <int BN>
+__device__ __forceinline__ TaPos ta_locate(const TaArgs& a, int64_t u) {
+  const int per = a.p.n_head_kv * a.row_tiles;
+  for (int b = 0; b < a.p.B; ++b) {
+    const TaSpan s = ta_span(a.p, b);
+    const int nblk = (s.hi - s.lo + BN - 1) / BN;
+    const int64_t here = (int64_t)nblk * per;
+    if (u < here) {
+      const int item = (int)(u / nblk);
+      return TaPos{b, item / a.row_tiles, item % a.row_tiles, (int)(u % nblk), nblk};
+    }
+    u -= here;
+  }
+  return TaPos{a.p.B, 0, 0, 0, 1};
+}
+
+template <int BN>
+__device__ __forceinline__ void ta_next(const TaArgs& a, TaPos& x) {
+  if (++x.blk < x.nblk) return;
+  x.blk = 0;
+  if (++x.rt < a.row_tiles) return;
+  x.rt = 0;
+  if (++x.h < a.p.n_head_kv) return;
+  x.h = 0;
+  do {
+    if (++x.b >= a.p.B) return;
+    const TaSpan s = ta_span(a.p, x.b);
+    x.nblk = (s.hi - s.lo + BN - 1) / BN;
+  } while (x.nblk == 0);
+}
+
+// ---- tensor-core products
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <int DT>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (DT == NS_F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo, both rounded to the 11 significant bits of tf32 (the tensor core drops the bits below)
+__device__ __forceinline__ void tf32_split(uint32_t x, uint32_t& hi, uint32_t& lo) {
+  hi = (x + 0x1000u) & 0xFFFFE000u;
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi)) + 0x1000u;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (DT == NS_F16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16-byte copy into shared memory, zeros when `ok` is false (nothing is read then).
+__device__ __forceinline__ void cp_async16_z(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
+template <int DT, int HD, int WM>
+__global__ void __launch_bounds__(kTaThreads, 1) tree_attn_kernel(const __grid_constant__ TaArgs a) {
+  using Cfg = TaCfg<DT, HD>;
+  constexpr int BN = Cfg::kBlock, EL = Cfg::kEl, RB = Cfg::kRowBytes;
+  constexpr int WK = kTaWarps / WM, MR = 16 * WM, KW = BN / WK, SB = KW < 32 ? KW : 32;
+  constexpr int CH = RB / 16;  // 16-byte chunks of a row
+  extern __shared__ __align__(128) uint8_t ta_smem[];
+  __shared__ TaShared S;
+  const ns_tree_attn_t& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int wm = warp % WM, wk = warp / WM;
+  const int g = lane >> 2, tq = lane & 3;
+  const uint32_t sbase = smem_addr(ta_smem);
+
+  griddep_wait();
+  griddep_launch_dependents();
+  const int64_t total = ta_total<BN>(a);
+  const int runs = ta_runs(a, total);
+  if ((int)blockIdx.x >= runs) return;
+  const int64_t u0 = ta_first_unit(total, runs, blockIdx.x), u1 = ta_first_unit(total, runs, blockIdx.x + 1);
+
+  TaPos ld = ta_locate<BN>(a, u0), at = ld;
+  const int row_chunks = p.head_dim * EL / 16;
+  auto load_block = [&](int stage) {  // the block at `ld` into a stage; rows past the end and dims past head_dim are zeros
+    const TaSpan s = ta_span(p, ld.b);
+    const int k0 = s.lo + ld.blk * BN;
+    const char* kb = static_cast<const char*>(p.k_cache) + (ld.b * p.kc_stride[0] + ld.h * p.kc_stride[1]) * EL;
+    const char* vb = static_cast<const char*>(p.v_cache) + (ld.b * p.vc_stride[0] + ld.h * p.vc_stride[1]) * EL;
+    const uint32_t dk = sbase + stage * 2 * Cfg::kTile, dv = dk + Cfg::kTile;
+#pragma unroll
+    for (int i = 0; i < BN * CH / kTaThreads; ++i) {
+      const int c = tid + i * kTaThreads, r = c / CH, ch = c % CH;
+      const bool ok = k0 + r < s.hi && ch < row_chunks;
+      const int64_t key = ok ? k0 + r : s.lo;
+      const int cc = ok ? ch : 0;
+      const uint32_t off = r * RB + ((ch ^ (r & 7)) << 4);
+      cp_async16_z(dk + off, kb + key * p.kc_stride[2] * EL + cc * 16, ok);
+      cp_async16_z(dv + off, vb + key * p.vc_stride[2] * EL + cc * 16, ok);
+    }
+  };
+
+  int64_t ul = u0;
+#pragma unroll
+  for (int i = 0; i < kTaStages - 1; ++i) {
+    if (ul < u1) {
+      load_block(i);
+      ta_next<BN>(a, ld);
+      ++ul;
+    }
+    cp_async_commit();
+  }
+
+  const float sc_hi = p.scale * 1.4426950408889634f;
+  const float sc_lo = fmaf(p.scale, 1.4426950408889634f, -sc_hi) + p.scale * 1.925963033500e-8f;
+
+  float o[HD / 8][4];
+  float m[2], l[2];
+  uint32_t qf[DT == NS_F32 ? 1 : HD / 16][4];
+  uint64_t anc[2] = {0, 0};
+  int dep[2] = {0, 0}, cur_b = -1;
+  bool fresh = true;
+  int first_blk = 0;
+
+  int stage = 0;
+  for (int64_t u = u0; u < u1; ++u) {
+    const TaSpan sp = ta_span(p, at.b);
+    if (fresh) {  // a new item: its tree and this thread's two rows
+      first_blk = at.blk;
+      if (at.b != cur_b) {
+        __syncthreads();
+        if (tid == 0) S.max_depth = 0;
+        __syncthreads();
+        if (tid < p.T) {
+          bool bad = false;
+          uint64_t mk = p.parents ? tree_mask(tid, [&](int i) { return p.parents[(int64_t)at.b * p.T + i]; }, &bad)
+                                  : chain_mask(tid);
+          if (mk && sp.len + tid >= p.max_ctx) mk = 0, bad = true;
+          if (bad) raise_device_error(NS_DEVERR_ROUTE);
+          S.anc[tid] = mk;
+          S.depth[tid] = __popcll(mk) - 1;
+          atomicMax(&S.max_depth, __popcll(mk) - 1);
+        }
+        __syncthreads();
+        cur_b = at.b;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = at.rt * MR + wm * 16 + g + 8 * i, t = r / a.rep;
+        anc[i] = t < p.T ? S.anc[t] : 0;
+        dep[i] = t < p.T ? S.depth[t] : 0;
+        m[i] = -INFINITY, l[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+      if constexpr (DT != NS_F32) {  // the rows' queries as A fragments, from global memory
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = at.rt * MR + wm * 16 + g + 8 * i, t = r / a.rep, hr = r % a.rep;
+          const uint16_t* q = static_cast<const uint16_t*>(p.q) + at.b * p.q_stride[0] + t * p.q_stride[1] +
+                              (at.h * a.rep + hr) * p.q_stride[2];
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+            for (int hlf = 0; hlf < 2; ++hlf) {
+              const int d = kk * 16 + hlf * 8 + 2 * tq;
+              uint32_t w = 0;
+              if (t < p.T && d < p.head_dim) w = (uint32_t)q[d] | ((uint32_t)q[d + 1] << 16);
+              qf[kk][hlf * 2 + i] = w;
+            }
+        }
+      }
+      fresh = false;
+    }
+
+    cp_async_wait<kTaStages - 2>();
+    __syncthreads();
+    // the next block goes into the stage that was used last, unless an item's end still needs it
+    const bool last_of_item = at.blk + 1 == at.nblk || u + 1 == u1;
+    const int free_stage = (stage + kTaStages - 1) % kTaStages;
+    if (ul < u1) {
+      load_block(free_stage);
+      ta_next<BN>(a, ld);
+      ++ul;
+    }
+    cp_async_commit();
+
+    const uint32_t ks = sbase + stage * 2 * Cfg::kTile, vs = ks + Cfg::kTile;
+    const int k0 = sp.lo + at.blk * BN;
+    // a block needs no mask when every row sees all of it
+    const bool masked = k0 + BN > sp.len || (p.window > 0 && sp.len + S.max_depth - k0 >= p.window);
+    if (masked) {
+      // values that not every row sees may hold anything: rows of the block that are not finite are
+      // set to zero here and added, for the rows that see them, from the cache below
+      if (tid < 4) S.bad_keys[tid] = 0;
+      __syncthreads();
+      for (int c = tid; c < BN * CH; c += kTaThreads) {
+        const int r = c / CH;
+        const uint32_t ad = vs + r * RB + (c % CH) * 16;
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w = lds32(ad + 4 * j);
+          if constexpr (DT == NS_F32) bad |= (w & 0x7F800000u) == 0x7F800000u;
+          else if constexpr (DT == NS_F16) bad |= (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
+          else bad |= (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+        }
+        if (bad) atomicOr(&S.bad_keys[r >> 5], 1u << (r & 31));
+      }
+      __syncthreads();
+      for (int c = tid; c < BN * CH; c += kTaThreads) {
+        const int r = c / CH;
+        if (S.bad_keys[r >> 5] >> (r & 31) & 1) sts128(vs + r * RB + (c % CH) * 16, 0, 0, 0, 0);
+      }
+      __syncthreads();
+    }
+
+#pragma unroll 1
+    for (int sb = 0; sb < KW / SB; ++sb) {
+      const int kr = wk * KW + sb * SB;  // first key row of the sub-block within the block
+      float s[SB / 8][4];
+#pragma unroll
+      for (int i = 0; i < SB / 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+      if constexpr (DT != NS_F32) {
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+          for (int n = 0; n < SB / 16; ++n) {  // 16 keys x 16 dims: two n-tiles of B fragments
+            uint32_t kf[4];
+            const int r = kr + n * 16 + (lane & 7) + ((lane >> 4) << 3), ch = kk * 2 + ((lane >> 3) & 1);
+            ldsm4(kf, ks + r * RB + ((ch ^ (r & 7)) << 4));
+            mma16<DT>(s[2 * n], qf[kk], kf[0], kf[1]);
+            mma16<DT>(s[2 * n + 1], qf[kk], kf[2], kf[3]);
+          }
+      } else {
+        const int r0 = at.rt * MR + wm * 16 + g;
+        const int t0 = r0 / a.rep, t1 = (r0 + 8) / a.rep;
+        const float* q0 = static_cast<const float*>(p.q) + at.b * p.q_stride[0] + t0 * p.q_stride[1] +
+                          (at.h * a.rep + r0 % a.rep) * p.q_stride[2];
+        const float* q1 = static_cast<const float*>(p.q) + at.b * p.q_stride[0] + t1 * p.q_stride[1] +
+                          (at.h * a.rep + (r0 + 8) % a.rep) * p.q_stride[2];
+#pragma unroll
+        for (int kk = 0; kk < HD / 8; ++kk) {
+          const int d = kk * 8 + tq;
+          uint32_t ah[4], al[4];
+          tf32_split(t0 < p.T && d < p.head_dim ? __float_as_uint(q0[d]) : 0u, ah[0], al[0]);
+          tf32_split(t1 < p.T && d < p.head_dim ? __float_as_uint(q1[d]) : 0u, ah[1], al[1]);
+          tf32_split(t0 < p.T && d + 4 < p.head_dim ? __float_as_uint(q0[d + 4]) : 0u, ah[2], al[2]);
+          tf32_split(t1 < p.T && d + 4 < p.head_dim ? __float_as_uint(q1[d + 4]) : 0u, ah[3], al[3]);
+#pragma unroll
+          for (int n = 0; n < SB / 8; ++n) {
+            const int r = kr + n * 8 + g;
+            uint32_t bh0, bl0, bh1, bl1;
+            tf32_split(lds32(ks + r * RB + (((2 * kk) ^ (r & 7)) << 4) + 4 * tq), bh0, bl0);
+            tf32_split(lds32(ks + r * RB + (((2 * kk + 1) ^ (r & 7)) << 4) + 4 * tq), bh1, bl1);
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            mma8(c, al, bh0, bh1);
+            mma8(c, ah, bl0, bl1);
+            mma8(c, ah, bh0, bh1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[n][j] += c[j];
+          }
+        }
+      }
+      // scores in units of log2, masked; running maximum
+      float mx[2] = {m[0], m[1]};
+      if (masked) {
+#pragma unroll
+        for (int n = 0; n < SB / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = k0 + kr + n * 8 + 2 * tq + (j & 1), i = j >> 1;
+            bool see;
+            if (key < sp.len) {
+              see = anc[i] != 0 && (p.window == 0 || sp.len + dep[i] - key < p.window);
+            } else {
+              const int nd = key - sp.len;
+              see = nd < p.T && nd < kTreeMax && (anc[i] >> nd & 1) &&
+                    (p.window == 0 || dep[i] - S.depth[nd] < p.window);
+            }
+            if (!see) s[n][j] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < SB / 8; ++n) {
+        mx[0] = fmaxf(mx[0], fmaxf(s[n][0], s[n][1]) * sc_hi);
+        mx[1] = fmaxf(mx[1], fmaxf(s[n][2], s[n][3]) * sc_hi);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      }
+      float corr[2], ref[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ref[i] = mx[i] == -INFINITY ? 0.f : mx[i];
+        corr[i] = ex2(m[i] - ref[i]);
+        m[i] = mx[i];
+        l[i] *= corr[i];
+      }
+#pragma unroll
+      for (int n = 0; n < SB / 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = s[n][j];
+          const float e = DT == NS_F32 && x != -INFINITY ? fmaf(x, sc_lo, fmaf(x, sc_hi, -ref[j >> 1]))
+                                                         : fmaf(x, sc_hi, -ref[j >> 1]);
+          s[n][j] = ex2(e);
+          l[j >> 1] += s[n][j];
+        }
+      if constexpr (DT != NS_F32) {
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          o[i][0] *= corr[0], o[i][1] *= corr[0];
+          o[i][2] *= corr[1], o[i][3] *= corr[1];
+        }
+#pragma unroll
+        for (int kk = 0; kk < SB / 16; ++kk) {
+          // probabilities rounded to 16 bits: half an ulp each, as large as the output's own rounding
+          const uint32_t pf[4] = {pack16<DT>(s[2 * kk][0], s[2 * kk][1]), pack16<DT>(s[2 * kk][2], s[2 * kk][3]),
+                                  pack16<DT>(s[2 * kk + 1][0], s[2 * kk + 1][1]),
+                                  pack16<DT>(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+          for (int n = 0; n < HD / 16; ++n) {
+            uint32_t vf[4];
+            const int r = kr + kk * 16 + (lane & 15), ch = n * 2 + (lane >> 4);
+            ldsm4_t(vf, vs + r * RB + ((ch ^ (r & 7)) << 4));
+            mma16<DT>(o[2 * n], pf, vf[0], vf[1]);
+            mma16<DT>(o[2 * n + 1], pf, vf[2], vf[3]);
+          }
+        }
+      } else {
+        // keys 2t and 2t+1 of an octet stand at k = t and t + 4, where the score fragments have them
+        uint32_t ph[SB / 8][4], pl[SB / 8][4];
+#pragma unroll
+        for (int kk = 0; kk < SB / 8; ++kk) {
+          tf32_split(__float_as_uint(s[kk][0]), ph[kk][0], pl[kk][0]);
+          tf32_split(__float_as_uint(s[kk][2]), ph[kk][1], pl[kk][1]);
+          tf32_split(__float_as_uint(s[kk][1]), ph[kk][2], pl[kk][2]);
+          tf32_split(__float_as_uint(s[kk][3]), ph[kk][3], pl[kk][3]);
+        }
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {
+#pragma unroll
+          for (int kk = 0; kk < SB / 8; ++kk) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            const int r = kr + kk * 8 + 2 * tq, ch = n * 2 + (g >> 2);
+            uint32_t bh0, bl0, bh1, bl1;
+            tf32_split(lds32(vs + r * RB + ((ch ^ (r & 7)) << 4) + 4 * (g & 3)), bh0, bl0);
+            tf32_split(lds32(vs + (r + 1) * RB + ((ch ^ ((r + 1) & 7)) << 4) + 4 * (g & 3)), bh1, bl1);
+            mma8(c, pl[kk], bh0, bh1);
+            mma8(c, ph[kk], bl0, bl1);
+            mma8(c, ph[kk], bh0, bh1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][j] = kk == 0 ? fmaf(o[n][j], corr[j >> 1], c[j]) : o[n][j] + c[j];
+          }
+        }
+      }
+      if (masked) {  // values that are not finite, for the rows that see them
+        uint32_t bad = S.bad_keys[kr >> 5] >> (kr & 31);
+        if constexpr (SB < 32) bad &= (1u << SB) - 1;
+        while (bad) {
+          const int kk = __ffs(bad) - 1;
+          bad &= bad - 1;
+          float pv[2] = {0.f, 0.f};
+#pragma unroll
+          for (int n = 0; n < SB / 8; ++n)
+            if (n == kk >> 3) pv[0] = kk & 1 ? s[n][1] : s[n][0], pv[1] = kk & 1 ? s[n][3] : s[n][2];
+          const int from = (lane & ~3) | ((kk & 7) >> 1);
+          pv[0] = __shfl_sync(0xffffffffu, pv[0], from);
+          pv[1] = __shfl_sync(0xffffffffu, pv[1], from);
+          const int64_t vrow = at.b * p.vc_stride[0] + at.h * p.vc_stride[1] + (int64_t)(k0 + kr + kk) * p.vc_stride[2];
+#pragma unroll
+          for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int d = n * 8 + 2 * tq + j;
+              if (d >= p.head_dim) continue;
+              const float v = load_float(p.v_cache, DT, vrow + d);
+              if (pv[0] != 0.f) o[n][j] = fmaf(pv[0], v, o[n][j]);
+              if (pv[1] != 0.f) o[n][2 + j] = fmaf(pv[1], v, o[n][2 + j]);
+            }
+        }
+      }
+    }
+
+    if (last_of_item) {
+      // the row sums of the quad; then the key groups join in order through the stage just consumed
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      }
+      const bool whole = first_blk == 0 && at.blk + 1 == at.nblk;
+      if constexpr (WK > 1) {
+        static_assert(kTaWarps * 16 * HD * 4 <= 2 * Cfg::kTile, "the join fits the stage");
+        __syncthreads();  // every warp is done with the stage
+        float* jo = reinterpret_cast<float*>(ta_smem + stage * 2 * Cfg::kTile);
+        if (tq == 0) {
+          S.wm[warp][g] = m[0], S.wm[warp][g + 8] = m[1];
+          S.wl[warp][g] = l[0], S.wl[warp][g + 8] = l[1];
+        }
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            jo[(warp * 16 + g + 8 * (j >> 1)) * HD + n * 8 + 2 * tq + (j & 1)] = o[n][j];
+        __syncthreads();
+      }
+      // rows leave as whole rows: a warp takes row after row
+      const int n_rows = min(MR, p.T * a.rep - at.rt * MR);
+      const int slot = 2 * blockIdx.x + (u - at.blk <= u0 ? 0 : 1);
+      if constexpr (WK > 1) {
+        const float* jo = reinterpret_cast<const float*>(ta_smem + stage * 2 * Cfg::kTile);
+        for (int r = warp; r < n_rows; r += kTaWarps) {
+          const int grp = r / 16, ri = r % 16;
+          float mt = -INFINITY, lt = 0.f, acc[HD / 32];
+#pragma unroll
+          for (int i = 0; i < HD / 32; ++i) acc[i] = 0.f;
+#pragma unroll
+          for (int w = 0; w < WK; ++w) mt = fmaxf(mt, S.wm[w * WM + grp][ri]);
+          const float ref = mt == -INFINITY ? 0.f : mt;
+#pragma unroll
+          for (int w = 0; w < WK; ++w) {
+            const float f = ex2(S.wm[w * WM + grp][ri] - ref);
+            lt = fmaf(S.wl[w * WM + grp][ri], f, lt);
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i)
+              acc[i] = fmaf(jo[((w * WM + grp) * 16 + ri) * HD + lane + 32 * i], f, acc[i]);
+          }
+          const int row = at.rt * MR + r, t = row / a.rep, h = at.h * a.rep + row % a.rep;
+          if (whole) {
+            const bool live = S.anc[t] != 0 && mt != -INFINITY;
+            float scale = 0.f;
+            if (live) {
+              if (p.sinks) {
+                const float sk = p.sinks[h] * 1.4426950408889634f, mm = fmaxf(mt, sk);
+                scale = ex2(mt - mm) / fmaf(lt, ex2(mt - mm), ex2(sk - mm));
+              } else {
+                scale = 1.f / lt;
+              }
+            }
+            const int64_t oo = at.b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i)
+              if (lane + 32 * i < p.head_dim) store_float(p.out, DT, oo + lane + 32 * i, live ? acc[i] * scale : 0.f);
+          } else {
+            float* po = a.part_o + ((int64_t)slot * MR + r) * HD;
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) po[lane + 32 * i] = acc[i];
+            if (lane == 0) {
+              a.part_ml[((int64_t)slot * MR + r) * 2] = mt;
+              a.part_ml[((int64_t)slot * MR + r) * 2 + 1] = lt;
+            }
+          }
+        }
+        __syncthreads();  // the stage may be filled again
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = wm * 16 + g + 8 * i;
+          if (r >= n_rows) continue;
+          const int row = at.rt * MR + r, t = row / a.rep, h = at.h * a.rep + row % a.rep;
+          if (whole) {
+            const bool live = anc[i] != 0 && m[i] != -INFINITY;
+            float scale = 0.f;
+            if (live) {
+              if (p.sinks) {
+                const float sk = p.sinks[h] * 1.4426950408889634f, mm = fmaxf(m[i], sk);
+                scale = ex2(m[i] - mm) / fmaf(l[i], ex2(m[i] - mm), ex2(sk - mm));
+              } else {
+                scale = 1.f / l[i];
+              }
+            }
+            const int64_t oo = at.b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int d = n * 8 + 2 * tq + j;
+                if (d < p.head_dim) store_float(p.out, DT, oo + d, live ? o[n][2 * i + j] * scale : 0.f);
+              }
+          } else {
+            float* po = a.part_o + ((int64_t)slot * MR + r) * HD;
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n)
+              *reinterpret_cast<float2*>(po + n * 8 + 2 * tq) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+            if (tq == 0) {
+              a.part_ml[((int64_t)slot * MR + r) * 2] = m[i];
+              a.part_ml[((int64_t)slot * MR + r) * 2 + 1] = l[i];
+            }
+          }
+        }
+      }
+      fresh = true;
+    }
+    ta_next<BN>(a, at);
+    stage = (stage + 1) % kTaStages;
+  }
+}
+
+// Joins the partial rows of items that were cut between runs, in order of the keys; a warp per row.
+// Rows that nothing was computed for (an empty or bad sequence) are zero.
+template <int DT, int HD, int WM>
+__global__ void __launch_bounds__(256) tree_attn_join_kernel(const __grid_constant__ TaArgs a) {
+  constexpr int BN = TaCfg<DT, HD>::kBlock, MR = 16 * WM;
+  const ns_tree_attn_t& p = a.p;
+  const int lane = threadIdx.x & 31;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int64_t total = ta_total<BN>(a);
+  const int runs = ta_runs(a, total);
+  const int64_t rows = (int64_t)p.B * p.T * p.n_head;
+  for (int64_t x = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); x < rows; x += (int64_t)gridDim.x * 8) {
+    const int b = (int)(x / ((int64_t)p.T * p.n_head)), rem = (int)(x % ((int64_t)p.T * p.n_head));
+    const int t = rem / p.n_head, h = rem % p.n_head, hk = h / a.rep;
+    const int row = t * a.rep + h % a.rep, rt = row / MR, r = row % MR;
+    int64_t before = 0;
+    for (int i = 0; i < b; ++i) {
+      const TaSpan s = ta_span(p, i);
+      before += (s.hi - s.lo + BN - 1) / BN;
+    }
+    const TaSpan sp = ta_span(p, b);
+    const int nblk = (sp.hi - sp.lo + BN - 1) / BN;
+    const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
+    if (nblk == 0) {
+      for (int d = lane; d < p.head_dim; d += 32) store_float(p.out, DT, oo + d, 0.f);
+      if (lane == 0 && (p.lens[b] < 0 || p.lens[b] > p.max_ctx)) raise_device_error(NS_DEVERR_ROUTE);
+      continue;
+    }
+    const int64_t s = (before * p.n_head_kv + (int64_t)hk * nblk) * a.row_tiles + (int64_t)rt * nblk, e = s + nblk;
+    const int i0 = (int)(((s + 1) * runs - 1) / total), i1 = (int)((e * runs - 1) / total);
+    if (i0 == i1) continue;  // one run covered it
+    bool bad = false;
+    const bool used = p.parents ? tree_mask(t, [&](int i) { return p.parents[(int64_t)b * p.T + i]; }, &bad) != 0 : true;
+    float mt = p.sinks ? p.sinks[h] * 1.4426950408889634f : -INFINITY, lt = p.sinks ? 1.f : 0.f, acc[HD / 32];
+    float mk = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) acc[i] = 0.f;
+    for (int i = i0; i <= i1; ++i) {
+      const int slot = 2 * i + (ta_first_unit(total, runs, i) >= s ? 0 : 1);
+      const int64_t base = (int64_t)slot * MR + r;
+      const float mi = a.part_ml[base * 2], li = a.part_ml[base * 2 + 1];
+      const float mn = fmaxf(mt, mi), ref = mn == -INFINITY ? 0.f : mn;
+      const float f = ex2(mt - ref), fi = ex2(mi - ref);
+      mk = fmaxf(mk, mi);
+      mt = mn;
+      lt = lt * f + li * fi;
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) acc[j] = acc[j] * f + a.part_o[base * HD + lane + 32 * j] * fi;
+    }
+    const bool live = used && mk != -INFINITY && sp.len + t < p.max_ctx;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j)
+      if (lane + 32 * j < p.head_dim) store_float(p.out, DT, oo + lane + 32 * j, live ? acc[j] / lt : 0.f);
+  }
+}
+
+// ---- host
+
+// Runs of a launch, at most: the workspace is sized for it without asking the device.
+constexpr int kTaMaxSms = 160;
+template <int DT, int HD>
+constexpr int ta_ctas_per_sm() { return 2 * (TaCfg<DT, HD>::kSmem + 2048) <= 227 * 1024 ? 2 : 1; }
+
+static int ta_groups(const ns_tree_attn_t* p) {  // WM: 16-row groups of a tile
+  const int rows = p->T * (p->n_head / p->n_head_kv);
+  return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
+}
+
+template <int DT, int HD, int WM>
+static int ta_run(const ns_tree_attn_t* p, void* ws, ns_stream_t stream, size_t* bytes) {
+  constexpr int MR = 16 * WM, max_grid = kTaMaxSms * ta_ctas_per_sm<DT, HD>();
+  const size_t o_bytes = (size_t)2 * max_grid * MR * HD * sizeof(float);
+  if (bytes) {
+    *bytes = o_bytes + (size_t)2 * max_grid * MR * 2 * sizeof(float);
+    return NS_OK;
+  }
+  TaArgs a;
+  a.p = *p;
+  a.rep = p->n_head / p->n_head_kv;
+  a.row_tiles = (p->T * a.rep + MR - 1) / MR;
+  a.part_o = static_cast<float*>(ws);
+  a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + o_bytes);
+  int sms = 0;
+  int st = num_sms(&sms);
+  if (st) return st;
+  const size_t smem = TaCfg<DT, HD>::kSmem;
+  NS_CUDA_TRY(cudaFuncSetAttribute(tree_attn_kernel<DT, HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  a.grid = std::min(sms, kTaMaxSms) * ta_ctas_per_sm<DT, HD>();
+  NS_CUDA_TRY(launch_pdl(tree_attn_kernel<DT, HD, WM>, dim3(a.grid), kTaThreads, smem, stream, 1, a));
+  const int64_t rows = (int64_t)p->B * p->T * p->n_head;
+  const int join = (int)std::min<int64_t>((rows + 7) / 8, 1 << 20);
+  NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, WM>, dim3(join), 256, 0, stream, 1, a));
+  return NS_OK;
+}
+
+template <int DT, int HD>
+static int ta_by_rows(const ns_tree_attn_t* p, void* ws, ns_stream_t stream, size_t* bytes) {
+  switch (ta_groups(p)) {
+    case 1: return ta_run<DT, HD, 1>(p, ws, stream, bytes);
+    case 2: return ta_run<DT, HD, 2>(p, ws, stream, bytes);
+    case 4: return ta_run<DT, HD, 4>(p, ws, stream, bytes);
+    default: return ta_run<DT, HD, 8>(p, ws, stream, bytes);
+  }
+}
+
+// Launches the call, or with `bytes` says what workspace it takes.
+static int ta_dispatch(const ns_tree_attn_t* p, void* ws, ns_stream_t stream, size_t* bytes) {
+  const bool wide = p->head_dim > 64;
+  switch (p->dtype) {
+    case NS_F32: return wide ? ta_by_rows<NS_F32, 128>(p, ws, stream, bytes) : ta_by_rows<NS_F32, 64>(p, ws, stream, bytes);
+    case NS_F16: return wide ? ta_by_rows<NS_F16, 128>(p, ws, stream, bytes) : ta_by_rows<NS_F16, 64>(p, ws, stream, bytes);
+    default: return wide ? ta_by_rows<NS_BF16, 128>(p, ws, stream, bytes) : ta_by_rows<NS_BF16, 64>(p, ws, stream, bytes);
+  }
+}
+
+static int ta_check(const ns_tree_attn_t* p) {
+  if (!p) return fail(NS_ERR_INVALID, "ns_tree_attn: null parameters");
+  if (p->B < 0 || p->T < 0 || p->max_ctx < 1 || p->window < 0)
+    return fail(NS_ERR_INVALID, "ns_tree_attn: B %d, T %d, max_ctx %d, window %d", p->B, p->T, p->max_ctx, p->window);
+  if (!float_type_ok(p->dtype)) return fail(NS_ERR_INVALID, "ns_tree_attn: bad dtype %d", p->dtype);
+  if (p->T > NS_TREE_MAX_NODES)
+    return fail(NS_ERR_UNSUPPORTED, "ns_tree_attn: %d nodes (at most %d)", p->T, NS_TREE_MAX_NODES);
+  if (p->head_dim < 8 || p->head_dim > 128 || p->head_dim % 8)
+    return fail(NS_ERR_UNSUPPORTED, "ns_tree_attn: head_dim %d (a multiple of 8 up to 128)", p->head_dim);
+  if (p->n_head_kv < 1 || p->n_head < 1 || p->n_head % p->n_head_kv)
+    return fail(NS_ERR_INVALID, "ns_tree_attn: %d query heads over %d kv heads", p->n_head, p->n_head_kv);
+  if (p->n_head > 65536 || p->B > (1 << 20))
+    return fail(NS_ERR_UNSUPPORTED, "ns_tree_attn: %d heads, %d sequences", p->n_head, p->B);
+  if (!(p->scale > 0.f) || p->scale > 3e38f) return fail(NS_ERR_INVALID, "ns_tree_attn: scale must be positive and finite");
+  return NS_OK;
+}
+
+}  // namespace ns
+
+extern "C" int ns_tree_attn_workspace_bytes(const ns_tree_attn_t* p, size_t* bytes) {
+  using namespace ns;
+  if (!bytes) return fail(NS_ERR_INVALID, "ns_tree_attn_workspace_bytes: null output");
+  int st = ta_check(p);
+  if (st) return st;
+  return ta_dispatch(p, nullptr, nullptr, bytes);
+}
+
+extern "C" int ns_tree_attn(const ns_tree_attn_t* p, void* workspace, size_t workspace_bytes, ns_stream_t stream) {
+  using namespace ns;
+  int st = ta_check(p);
+  if (st) return st;
+  if (p->B == 0 || p->T == 0) return NS_OK;
+  if (!p->lens || !p->q || !p->k_cache || !p->v_cache || !p->out || !workspace)
+    return fail(NS_ERR_INVALID, "ns_tree_attn: null pointer");
+  const int64_t m = p->dtype == NS_F32 ? 4 : 8;
+  if (!aligned_to(p->k_cache, 16) || !aligned_to(p->v_cache, 16) || !strides_multiple(p->kc_stride, 3, m) ||
+      !strides_multiple(p->vc_stride, 3, m))
+    return fail(NS_ERR_INVALID, "ns_tree_attn: caches must start and step by 16 bytes");
+  if (!aligned_to(workspace, 256)) return fail(NS_ERR_INVALID, "ns_tree_attn: workspace must be 256-byte aligned");
+  size_t need = 0;
+  st = ta_dispatch(p, nullptr, nullptr, &need);
+  if (st) return st;
+  if (workspace_bytes < need)
+    return fail(NS_ERR_SIZE, "ns_tree_attn: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  return ta_dispatch(p, workspace, stream, nullptr);
+}
