@@ -34,6 +34,7 @@ struct TaCfg {
   static constexpr int kRowBytes = HD * kEl;
   static constexpr int kTile = kBlock * kRowBytes;        // bytes of a key (or value) block
   static constexpr int kSmem = kTaStages * 2 * kTile;
+  static constexpr int kCtas = 2 * (kSmem + 4096) <= 227 * 1024 ? 2 : 1;  // of one SM
 };
 
 struct TaArgs {
@@ -168,10 +169,10 @@ __device__ __forceinline__ void cp_async16_z(uint32_t dst, const void* src, bool
 }
 
 template <int DT, int HD, int WM>
-__global__ void __launch_bounds__(kTaThreads, 1) tree_attn_kernel(const __grid_constant__ TaArgs a) {
+__global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_kernel(const __grid_constant__ TaArgs a) {
   using Cfg = TaCfg<DT, HD>;
   constexpr int BN = Cfg::kBlock, EL = Cfg::kEl, RB = Cfg::kRowBytes;
-  constexpr int WK = kTaWarps / WM, MR = 16 * WM, KW = BN / WK, SB = KW < 32 ? KW : 32;
+  constexpr int WK = kTaWarps / WM, MR = 16 * WM, KW = BN / WK, SB = DT == NS_F32 ? (KW < 16 ? KW : 16) : (KW < 32 ? KW : 32);
   constexpr int CH = RB / 16;  // 16-byte chunks of a row
   extern __shared__ __align__(128) uint8_t ta_smem[];
   __shared__ TaShared S;
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(kTaThreads, 1) tree_attn_kernel(const __grid_c
 
   float o[HD / 8][4];
   float m[2], l[2];
-  uint32_t qf[DT == NS_F32 ? 1 : HD / 16][4];
+  uint32_t qf[DT == NS_F32 ? HD / 8 : HD / 16][4];  // this warp's queries as A fragments
   uint64_t anc[2] = {0, 0};
   int dep[2] = {0, 0}, cur_b = -1;
   bool fresh = true;
@@ -263,12 +264,12 @@ __global__ void __launch_bounds__(kTaThreads, 1) tree_attn_kernel(const __grid_c
       for (int i = 0; i < HD / 8; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-      if constexpr (DT != NS_F32) {  // the rows' queries as A fragments, from global memory
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = at.rt * MR + wm * 16 + g + 8 * i, t = r / a.rep, hr = r % a.rep;
-          const uint16_t* q = static_cast<const uint16_t*>(p.q) + at.b * p.q_stride[0] + t * p.q_stride[1] +
-                              (at.h * a.rep + hr) * p.q_stride[2];
+      for (int i = 0; i < 2; ++i) {
+        const int r = at.rt * MR + wm * 16 + g + 8 * i, t = r / a.rep, hr = r % a.rep;
+        const int64_t qo = at.b * p.q_stride[0] + t * p.q_stride[1] + (at.h * a.rep + hr) * p.q_stride[2];
+        if constexpr (DT != NS_F32) {
+          const uint16_t* q = static_cast<const uint16_t*>(p.q) + qo;
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
 #pragma unroll
@@ -277,6 +278,15 @@ __global__ void __launch_bounds__(kTaThreads, 1) tree_attn_kernel(const __grid_c
               uint32_t w = 0;
               if (t < p.T && d < p.head_dim) w = (uint32_t)q[d] | ((uint32_t)q[d + 1] << 16);
               qf[kk][hlf * 2 + i] = w;
+            }
+        } else {
+          const float* q = static_cast<const float*>(p.q) + qo;
+#pragma unroll
+          for (int kk = 0; kk < HD / 8; ++kk)
+#pragma unroll
+            for (int hlf = 0; hlf < 2; ++hlf) {
+              const int d = kk * 8 + hlf * 4 + tq;
+              qf[kk][hlf * 2 + i] = t < p.T && d < p.head_dim ? __float_as_uint(q[d]) : 0u;
             }
         }
       }
@@ -345,20 +355,11 @@ __global__ void __launch_bounds__(kTaThreads, 1) tree_attn_kernel(const __grid_c
             mma16<DT>(s[2 * n + 1], qf[kk], kf[2], kf[3]);
           }
       } else {
-        const int r0 = at.rt * MR + wm * 16 + g;
-        const int t0 = r0 / a.rep, t1 = (r0 + 8) / a.rep;
-        const float* q0 = static_cast<const float*>(p.q) + at.b * p.q_stride[0] + t0 * p.q_stride[1] +
-                          (at.h * a.rep + r0 % a.rep) * p.q_stride[2];
-        const float* q1 = static_cast<const float*>(p.q) + at.b * p.q_stride[0] + t1 * p.q_stride[1] +
-                          (at.h * a.rep + (r0 + 8) % a.rep) * p.q_stride[2];
 #pragma unroll
         for (int kk = 0; kk < HD / 8; ++kk) {
-          const int d = kk * 8 + tq;
           uint32_t ah[4], al[4];
-          tf32_split(t0 < p.T && d < p.head_dim ? __float_as_uint(q0[d]) : 0u, ah[0], al[0]);
-          tf32_split(t1 < p.T && d < p.head_dim ? __float_as_uint(q1[d]) : 0u, ah[1], al[1]);
-          tf32_split(t0 < p.T && d + 4 < p.head_dim ? __float_as_uint(q0[d + 4]) : 0u, ah[2], al[2]);
-          tf32_split(t1 < p.T && d + 4 < p.head_dim ? __float_as_uint(q1[d + 4]) : 0u, ah[3], al[3]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tf32_split(qf[kk][j], ah[j], al[j]);
 #pragma unroll
           for (int n = 0; n < SB / 8; ++n) {
             const int r = kr + n * 8 + g;
@@ -612,60 +613,129 @@ __global__ void __launch_bounds__(kTaThreads, 1) tree_attn_kernel(const __grid_c
   }
 }
 
-// Joins the partial rows of items that were cut between runs, in order of the keys; a warp per row.
+// Joins the partial rows of items that were cut between runs, WPR warps per row; each warp takes a
+// contiguous share of the row's parts, the shares join in order: a result does not depend on timing.
 // Rows that nothing was computed for (an empty or bad sequence) are zero.
-template <int DT, int HD, int WM>
-__global__ void __launch_bounds__(256) tree_attn_join_kernel(const __grid_constant__ TaArgs a) {
-  constexpr int BN = TaCfg<DT, HD>::kBlock, MR = 16 * WM;
+constexpr int kJoinWarps = 8;
+
+template <int DT, int HD, int WM, int WPR>
+__global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const __grid_constant__ TaArgs a) {
+  constexpr int BN = TaCfg<DT, HD>::kBlock, MR = 16 * WM, V = HD / 32, RPC = kJoinWarps / WPR;
+  __shared__ float so[WPR > 1 ? kJoinWarps : 1][HD], sm[kJoinWarps], sl[kJoinWarps];
   const ns_tree_attn_t& p = a.p;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % WPR;
   griddep_wait();
   griddep_launch_dependents();
   const int64_t total = ta_total<BN>(a);
   const int runs = ta_runs(a, total);
   const int64_t rows = (int64_t)p.B * p.T * p.n_head;
-  for (int64_t x = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); x < rows; x += (int64_t)gridDim.x * 8) {
-    const int b = (int)(x / ((int64_t)p.T * p.n_head)), rem = (int)(x % ((int64_t)p.T * p.n_head));
-    const int t = rem / p.n_head, h = rem % p.n_head, hk = h / a.rep;
-    const int row = t * a.rep + h % a.rep, rt = row / MR, r = row % MR;
-    int64_t before = 0;
-    for (int i = 0; i < b; ++i) {
-      const TaSpan s = ta_span(p, i);
-      before += (s.hi - s.lo + BN - 1) / BN;
-    }
-    const TaSpan sp = ta_span(p, b);
-    const int nblk = (sp.hi - sp.lo + BN - 1) / BN;
-    const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
-    if (nblk == 0) {
-      for (int d = lane; d < p.head_dim; d += 32) store_float(p.out, DT, oo + d, 0.f);
-      if (lane == 0 && (p.lens[b] < 0 || p.lens[b] > p.max_ctx)) raise_device_error(NS_DEVERR_ROUTE);
-      continue;
-    }
-    const int64_t s = (before * p.n_head_kv + (int64_t)hk * nblk) * a.row_tiles + (int64_t)rt * nblk, e = s + nblk;
-    const int i0 = (int)(((s + 1) * runs - 1) / total), i1 = (int)((e * runs - 1) / total);
-    if (i0 == i1) continue;  // one run covered it
-    bool bad = false;
-    const bool used = p.parents ? tree_mask(t, [&](int i) { return p.parents[(int64_t)b * p.T + i]; }, &bad) != 0 : true;
-    float mt = p.sinks ? p.sinks[h] * 1.4426950408889634f : -INFINITY, lt = p.sinks ? 1.f : 0.f, acc[HD / 32];
-    float mk = -INFINITY;
+  for (int64_t x0 = (int64_t)blockIdx.x * RPC; x0 < rows; x0 += (int64_t)gridDim.x * RPC) {
+    const int64_t x = x0 + warp / WPR;
+    bool cut = false;
+    int b = 0, t = 0, h = 0;
+    TaSpan sp{0, 0, 0};
+    float mt = -INFINITY, lt = 0.f, acc[V];
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) acc[i] = 0.f;
-    for (int i = i0; i <= i1; ++i) {
-      const int slot = 2 * i + (ta_first_unit(total, runs, i) >= s ? 0 : 1);
-      const int64_t base = (int64_t)slot * MR + r;
-      const float mi = a.part_ml[base * 2], li = a.part_ml[base * 2 + 1];
-      const float mn = fmaxf(mt, mi), ref = mn == -INFINITY ? 0.f : mn;
-      const float f = ex2(mt - ref), fi = ex2(mi - ref);
-      mk = fmaxf(mk, mi);
-      mt = mn;
-      lt = lt * f + li * fi;
+    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+    if (x < rows) {
+      b = (int)(x / ((int64_t)p.T * p.n_head));
+      const int rem = (int)(x % ((int64_t)p.T * p.n_head));
+      t = rem / p.n_head, h = rem % p.n_head;
+      const int hk = h / a.rep, row = t * a.rep + h % a.rep, rt = row / MR, r = row % MR;
+      int64_t before = 0;
+      for (int i = 0; i < b; ++i) {
+        const TaSpan s = ta_span(p, i);
+        before += (s.hi - s.lo + BN - 1) / BN;
+      }
+      sp = ta_span(p, b);
+      const int nblk = (sp.hi - sp.lo + BN - 1) / BN;
+      if (nblk == 0) {
+        const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
+        if (share == 0)
+          for (int d = lane; d < p.head_dim; d += 32) store_float(p.out, DT, oo + d, 0.f);
+        if (lane == 0 && (p.lens[b] < 0 || p.lens[b] > p.max_ctx)) raise_device_error(NS_DEVERR_ROUTE);
+      } else {
+        const int64_t s = (before * p.n_head_kv + (int64_t)hk * nblk) * a.row_tiles + (int64_t)rt * nblk, e = s + nblk;
+        const int i0 = (int)(((s + 1) * runs - 1) / total), i1 = (int)((e * runs - 1) / total);
+        cut = i0 != i1;  // else one run covered it
+        if (cut) {
+          const int n = i1 - i0 + 1, from = i0 + n * share / WPR, to = i0 + n * (share + 1) / WPR;
+          for (int c = from; c < to; c += 32) {
+            float mi = -INFINITY, li = 0.f;
+            int64_t base = 0;
+            if (c + lane < to) {
+              const int slot = 2 * (c + lane) + (ta_first_unit(total, runs, c + lane) >= s ? 0 : 1);
+              base = (int64_t)slot * MR + r;
+              const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + base * 2);
+              mi = ml.x, li = ml.y;
+            }
+            float mn = fmaxf(mt, mi);
 #pragma unroll
-      for (int j = 0; j < HD / 32; ++j) acc[j] = acc[j] * f + a.part_o[base * HD + lane + 32 * j] * fi;
+            for (int o = 16; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+            const float ref = mn == -INFINITY ? 0.f : mn;
+            const float f = ex2(mt - ref), fi = ex2(mi - ref);
+            mt = mn;
+            lt = lt * f + warp_sum(li * fi);
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] *= f;
+            const int m = min(32, to - c);
+            for (int i = 0; i < m; i += 8) {
+              float v[8][V];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const int64_t at = __shfl_sync(0xffffffffu, base, (i + k) & 31);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[k][j] = i + k < m ? a.part_o[at * HD + lane + 32 * j] : 0.f;
+              }
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float fk = __shfl_sync(0xffffffffu, fi, (i + k) & 31);
+#pragma unroll
+                for (int j = 0; j < V; ++j) acc[j] = i + k < m ? fmaf(v[k][j], fk, acc[j]) : acc[j];
+              }
+            }
+          }
+        }
+      }
     }
-    const bool live = used && mk != -INFINITY && sp.len + t < p.max_ctx;
+    if constexpr (WPR > 1) {
 #pragma unroll
-    for (int j = 0; j < HD / 32; ++j)
-      if (lane + 32 * j < p.head_dim) store_float(p.out, DT, oo + lane + 32 * j, live ? acc[j] / lt : 0.f);
+      for (int j = 0; j < V; ++j) so[warp][lane + 32 * j] = acc[j];
+      if (lane == 0) sm[warp] = mt, sl[warp] = lt;
+      __syncthreads();
+      if (share == 0) {
+        float mn = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) mn = fmaxf(mn, sm[warp + w]);
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        lt = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] = 0.f;
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) {
+          const float f = ex2(sm[warp + w] - ref);
+          lt = fmaf(sl[warp + w], f, lt);
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[j] = fmaf(so[warp + w][lane + 32 * j], f, acc[j]);
+        }
+        mt = mn;
+      }
+    }
+    if (cut && share == 0) {
+      bool bad = false;
+      const bool used = p.parents ? tree_mask(t, [&](int i) { return p.parents[(int64_t)b * p.T + i]; }, &bad) != 0 : true;
+      const bool live = used && mt != -INFINITY && sp.len + t < p.max_ctx;
+      float scale = live ? 1.f / lt : 0.f;
+      if (live && p.sinks) {
+        const float sk = p.sinks[h] * 1.4426950408889634f, mm = fmaxf(mt, sk);
+        scale = ex2(mt - mm) / fmaf(lt, ex2(mt - mm), ex2(sk - mm));
+      }
+      const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (lane + 32 * j < p.head_dim) store_float(p.out, DT, oo + lane + 32 * j, live ? acc[j] * scale : 0.f);
+    }
+    if constexpr (WPR > 1) __syncthreads();
   }
 }
 
@@ -673,8 +743,6 @@ __global__ void __launch_bounds__(256) tree_attn_join_kernel(const __grid_consta
 
 // Runs of a launch, at most: the workspace is sized for it without asking the device.
 constexpr int kTaMaxSms = 160;
-template <int DT, int HD>
-constexpr int ta_ctas_per_sm() { return 2 * (TaCfg<DT, HD>::kSmem + 2048) <= 227 * 1024 ? 2 : 1; }
 
 static int ta_groups(const ns_tree_attn_t* p) {  // WM: 16-row groups of a tile
   const int rows = p->T * (p->n_head / p->n_head_kv);
@@ -683,7 +751,7 @@ static int ta_groups(const ns_tree_attn_t* p) {  // WM: 16-row groups of a tile
 
 template <int DT, int HD, int WM>
 static int ta_run(const ns_tree_attn_t* p, void* ws, ns_stream_t stream, size_t* bytes) {
-  constexpr int MR = 16 * WM, max_grid = kTaMaxSms * ta_ctas_per_sm<DT, HD>();
+  constexpr int MR = 16 * WM, max_grid = kTaMaxSms * TaCfg<DT, HD>::kCtas;
   const size_t o_bytes = (size_t)2 * max_grid * MR * HD * sizeof(float);
   if (bytes) {
     *bytes = o_bytes + (size_t)2 * max_grid * MR * 2 * sizeof(float);
@@ -700,11 +768,14 @@ static int ta_run(const ns_tree_attn_t* p, void* ws, ns_stream_t stream, size_t*
   if (st) return st;
   const size_t smem = TaCfg<DT, HD>::kSmem;
   NS_CUDA_TRY(cudaFuncSetAttribute(tree_attn_kernel<DT, HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  a.grid = std::min(sms, kTaMaxSms) * ta_ctas_per_sm<DT, HD>();
+  a.grid = std::min(sms, kTaMaxSms) * TaCfg<DT, HD>::kCtas;
   NS_CUDA_TRY(launch_pdl(tree_attn_kernel<DT, HD, WM>, dim3(a.grid), kTaThreads, smem, stream, 1, a));
   const int64_t rows = (int64_t)p->B * p->T * p->n_head;
-  const int join = (int)std::min<int64_t>((rows + 7) / 8, 1 << 20);
-  NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, WM>, dim3(join), 256, 0, stream, 1, a));
+  if (rows <= 1024)  // few rows: their many parts are shared out among the warps
+    NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, WM, kJoinWarps>, dim3((unsigned)rows), kJoinWarps * 32, 0, stream, 1, a));
+  else
+    NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, WM, 1>, dim3((unsigned)std::min<int64_t>((rows + 7) / 8, 1 << 20)),
+                           kJoinWarps * 32, 0, stream, 1, a));
   return NS_OK;
 }
 
