@@ -40,7 +40,9 @@ struct TaCfg {
 struct TaArgs {
   ns_tree_attn_t p;
   int rep;         // query heads per kv head
+  int tile_rows;   // rows of a tile
   int row_tiles;   // tiles of rows of one (sequence, kv head)
+  int block;       // keys of a block
   int grid;        // runs, at most: none is empty (ta_runs)
   float* part_o;   // [2 * grid][rows per tile][HD]
   float* part_ml;  // [2 * grid][rows per tile][2]
@@ -75,8 +77,7 @@ __device__ __forceinline__ int ta_runs(const TaArgs& a, int64_t total) { return 
 __device__ __forceinline__ int64_t ta_first_unit(int64_t total, int runs, int i) { return total * i / runs; }
 
 // The sequence and offset of unit u, by a walk over the sequences (all threads alike).
-template <int BN>
-__device__ __forceinline__ int64_t ta_total(const TaArgs& a) {
+__device__ __forceinline__ int64_t ta_total(const TaArgs& a, int BN) {
   int64_t n = 0;
   for (int b = 0; b < a.p.B; ++b) {
     const TaSpan s = ta_span(a.p, b);
@@ -85,8 +86,7 @@ __device__ __forceinline__ int64_t ta_total(const TaArgs& a) {
   return n * a.p.n_head_kv * a.row_tiles;
 }
 
-template <int BN>
-__device__ __forceinline__ TaPos ta_locate(const TaArgs& a, int64_t u) {
+__device__ __forceinline__ TaPos ta_locate(const TaArgs& a, int BN, int64_t u) {
   const int per = a.p.n_head_kv * a.row_tiles;
   for (int b = 0; b < a.p.B; ++b) {
     const TaSpan s = ta_span(a.p, b);
@@ -101,8 +101,7 @@ __device__ __forceinline__ TaPos ta_locate(const TaArgs& a, int64_t u) {
   return TaPos{a.p.B, 0, 0, 0, 1};
 }
 
-template <int BN>
-__device__ __forceinline__ void ta_next(const TaArgs& a, TaPos& x) {
+__device__ __forceinline__ void ta_next(const TaArgs& a, int BN, TaPos& x) {
   if (++x.blk < x.nblk) return;
   x.blk = 0;
   if (++x.rt < a.row_tiles) return;
@@ -184,12 +183,12 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
 
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t total = ta_total<BN>(a);
+  const int64_t total = ta_total(a, BN);
   const int runs = ta_runs(a, total);
   if ((int)blockIdx.x >= runs) return;
   const int64_t u0 = ta_first_unit(total, runs, blockIdx.x), u1 = ta_first_unit(total, runs, blockIdx.x + 1);
 
-  TaPos ld = ta_locate<BN>(a, u0), at = ld;
+  TaPos ld = ta_locate(a, BN, u0), at = ld;
   const int row_chunks = p.head_dim * EL / 16;
   auto load_block = [&](int stage) {  // the block at `ld` into a stage; rows past the end and dims past head_dim are zeros
     const TaSpan s = ta_span(p, ld.b);
@@ -214,7 +213,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
   for (int i = 0; i < kTaStages - 1; ++i) {
     if (ul < u1) {
       load_block(i);
-      ta_next<BN>(a, ld);
+      ta_next(a, BN, ld);
       ++ul;
     }
     cp_async_commit();
@@ -300,7 +299,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
     const int free_stage = (stage + kTaStages - 1) % kTaStages;
     if (ul < u1) {
       load_block(free_stage);
-      ta_next<BN>(a, ld);
+      ta_next(a, BN, ld);
       ++ul;
     }
     cp_async_commit();
@@ -608,7 +607,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
       }
       fresh = true;
     }
-    ta_next<BN>(a, at);
+    ta_next(a, BN, at);
     stage = (stage + 1) % kTaStages;
   }
 }
@@ -618,15 +617,16 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
 // Rows that nothing was computed for (an empty or bad sequence) are zero.
 constexpr int kJoinWarps = 8;
 
-template <int DT, int HD, int WM, int WPR>
+template <int DT, int HD, int WPR>
 __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const __grid_constant__ TaArgs a) {
-  constexpr int BN = TaCfg<DT, HD>::kBlock, MR = 16 * WM, V = HD / 32, RPC = kJoinWarps / WPR;
+  constexpr int V = HD / 32, RPC = kJoinWarps / WPR;
+  const int BN = a.block, MR = a.tile_rows;
   __shared__ float so[WPR > 1 ? kJoinWarps : 1][HD], sm[kJoinWarps], sl[kJoinWarps];
   const ns_tree_attn_t& p = a.p;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % WPR;
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t total = ta_total<BN>(a);
+  const int64_t total = ta_total(a, BN);
   const int runs = ta_runs(a, total);
   const int64_t rows = (int64_t)p.B * p.T * p.n_head;
   for (int64_t x0 = (int64_t)blockIdx.x * RPC; x0 < rows; x0 += (int64_t)gridDim.x * RPC) {
@@ -749,6 +749,17 @@ static int ta_groups(const ns_tree_attn_t* p) {  // WM: 16-row groups of a tile
   return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
 }
 
+template <int DT, int HD>
+static int ta_join(const TaArgs& a, ns_stream_t stream) {
+  const int64_t rows = (int64_t)a.p.B * a.p.T * a.p.n_head;
+  if (rows <= 1024)  // few rows: their many parts are shared out among the warps
+    NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, kJoinWarps>, dim3((unsigned)rows), kJoinWarps * 32, 0, stream, 1, a));
+  else
+    NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, 1>, dim3((unsigned)std::min<int64_t>((rows + 7) / 8, 1 << 20)),
+                           kJoinWarps * 32, 0, stream, 1, a));
+  return NS_OK;
+}
+
 template <int DT, int HD, int WM>
 static int ta_run(const ns_tree_attn_t* p, void* ws, ns_stream_t stream, size_t* bytes) {
   constexpr int MR = 16 * WM, max_grid = kTaMaxSms * TaCfg<DT, HD>::kCtas;
@@ -760,7 +771,9 @@ static int ta_run(const ns_tree_attn_t* p, void* ws, ns_stream_t stream, size_t*
   TaArgs a;
   a.p = *p;
   a.rep = p->n_head / p->n_head_kv;
+  a.tile_rows = MR;
   a.row_tiles = (p->T * a.rep + MR - 1) / MR;
+  a.block = TaCfg<DT, HD>::kBlock;
   a.part_o = static_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + o_bytes);
   int sms = 0;
@@ -770,17 +783,15 @@ static int ta_run(const ns_tree_attn_t* p, void* ws, ns_stream_t stream, size_t*
   NS_CUDA_TRY(cudaFuncSetAttribute(tree_attn_kernel<DT, HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   a.grid = std::min(sms, kTaMaxSms) * TaCfg<DT, HD>::kCtas;
   NS_CUDA_TRY(launch_pdl(tree_attn_kernel<DT, HD, WM>, dim3(a.grid), kTaThreads, smem, stream, 1, a));
-  const int64_t rows = (int64_t)p->B * p->T * p->n_head;
-  if (rows <= 1024)  // few rows: their many parts are shared out among the warps
-    NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, WM, kJoinWarps>, dim3((unsigned)rows), kJoinWarps * 32, 0, stream, 1, a));
-  else
-    NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, WM, 1>, dim3((unsigned)std::min<int64_t>((rows + 7) / 8, 1 << 20)),
-                           kJoinWarps * 32, 0, stream, 1, a));
-  return NS_OK;
+  return ta_join<DT, HD>(a, stream);
 }
+
+#include "tree_attn_tc.cuh"
 
 template <int DT, int HD>
 static int ta_by_rows(const ns_tree_attn_t* p, void* ws, ns_stream_t stream, size_t* bytes) {
+  if constexpr (DT != NS_F32)
+    if (ta_takes_tc(p)) return ta_run_tc<DT, HD>(p, ws, stream, bytes);
   switch (ta_groups(p)) {
     case 1: return ta_run<DT, HD, 1>(p, ws, stream, bytes);
     case 2: return ta_run<DT, HD, 2>(p, ws, stream, bytes);
