@@ -612,131 +612,169 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
   }
 }
 
-// Joins the partial rows of items that were cut between runs, WPR warps per row; each warp takes a
-// contiguous share of the row's parts, the shares join in order: a result does not depend on timing.
+// Joins the partial rows of items that were cut between runs.  A block takes a few rows of one item; the
+// item's place in the list, and so which runs hold its parts, is worked out once.  WPR = 1: a warp
+// takes whole rows, two or three parts each.  WPR = 8: few rows and many parts, a row's parts are shared
+// among the block's warps.  The order of the sums is fixed: a result does not depend on timing.
 // Rows that nothing was computed for (an empty or bad sequence) are zero.
 constexpr int kJoinWarps = 8;
+constexpr int kJoinRows = 4;  // rows a warp takes with WPR = 1
 
 template <int DT, int HD, int WPR>
 __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const __grid_constant__ TaArgs a) {
-  constexpr int V = HD / 32, RPC = kJoinWarps / WPR;
+  constexpr int V = HD / 32, RB = WPR == 1 ? kJoinWarps * kJoinRows : 1;
   const int BN = a.block, MR = a.tile_rows;
-  __shared__ float so[WPR > 1 ? kJoinWarps : 1][HD], sm[kJoinWarps], sl[kJoinWarps];
+  __shared__ float so[WPR > 1 ? WPR : 1][HD], sm[WPR], sl[WPR];
   const ns_tree_attn_t& p = a.p;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % WPR;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int item = blockIdx.x, rt = item % a.row_tiles, hk = item / a.row_tiles % p.n_head_kv;
+  const int b = item / a.row_tiles / p.n_head_kv;
+  const int n_rows = min(MR, p.T * a.rep - rt * MR);
+  const int r0 = blockIdx.y * RB;
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t total = ta_total(a, BN);
+  if (r0 >= n_rows) return;
+  // blocks of all sequences, and of those before this one
+  int64_t total = 0, before = 0;
+  for (int i = lane; i < p.B; i += 32) {
+    const TaSpan s = ta_span(p, i);
+    const int n = (s.hi - s.lo + BN - 1) / BN;
+    total += n;
+    if (i < b) before += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  total *= (int64_t)p.n_head_kv * a.row_tiles;
   const int runs = ta_runs(a, total);
-  const int64_t rows = (int64_t)p.B * p.T * p.n_head;
-  for (int64_t x0 = (int64_t)blockIdx.x * RPC; x0 < rows; x0 += (int64_t)gridDim.x * RPC) {
-    const int64_t x = x0 + warp / WPR;
-    bool cut = false;
-    int b = 0, t = 0, h = 0;
-    TaSpan sp{0, 0, 0};
+  const TaSpan sp = ta_span(p, b);
+  const int nblk = (sp.hi - sp.lo + BN - 1) / BN;
+  const int64_t s = (before * p.n_head_kv + (int64_t)hk * nblk) * a.row_tiles + (int64_t)rt * nblk, e = s + nblk;
+  const int i0 = nblk ? (int)(((s + 1) * runs - 1) / total) : 0, i1 = nblk ? (int)((e * runs - 1) / total) : 0;
+  if (nblk && i0 == i1) return;  // one run covered it
+  const int n = i1 - i0 + 1;
+
+  auto finish = [&](int r, float mt, float lt, float (&acc)[V]) {  // one row out
+    const int row = rt * MR + r, t = row / a.rep, h = hk * a.rep + row % a.rep;
+    bool bad = false;
+    const bool used = p.parents ? tree_mask(t, [&](int i) { return p.parents[(int64_t)b * p.T + i]; }, &bad) != 0 : true;
+    const bool live = nblk && used && mt != -INFINITY && sp.len + t < p.max_ctx;
+    float scale = live ? 1.f / lt : 0.f;
+    if (live && p.sinks) {
+      const float sk = p.sinks[h] * 1.4426950408889634f, mm = fmaxf(mt, sk);
+      scale = ex2(mt - mm) / fmaf(lt, ex2(mt - mm), ex2(sk - mm));
+    }
+    const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2] + lane * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = live ? acc[j] * scale : 0.f;
+    if constexpr (DT != NS_F32 && V == 4) {
+      uint16_t* out = static_cast<uint16_t*>(p.out) + oo;
+      if ((reinterpret_cast<uintptr_t>(out) & 7) == 0 && lane * V + V <= p.head_dim) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack16<DT>(acc[0], acc[1]), pack16<DT>(acc[2], acc[3]));
+        return;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (lane * V + j < p.head_dim) store_float(p.out, DT, oo + j, acc[j]);
+  };
+  auto load_part = [&](int64_t at, float (&v)[V]) {
+    const float* src = a.part_o + at * HD + lane * V;
+    if constexpr (V == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(src);
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(src);
+      v[0] = x.x, v[1] = x.y;
+    }
+  };
+
+  if constexpr (WPR == 1) {
+    for (int k = 0; k < kJoinRows; ++k) {
+      const int r = r0 + k * kJoinWarps + warp;
+      if (r >= n_rows) return;
+      float mt = -INFINITY, lt = 0.f, acc[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] = 0.f;
+      if (nblk)
+        for (int i = 0; i < n; ++i) {
+          const int64_t at = (int64_t)(2 * (i0 + i) + (i == 0 && ta_first_unit(total, runs, i0) < s ? 1 : 0)) * MR + r;
+          const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+          float v[V];
+          load_part(at, v);
+          const float mn = fmaxf(mt, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+          const float f = ex2(mt - ref), fi = ex2(ml.x - ref);
+          mt = mn;
+          lt = lt * f + ml.y * fi;
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[j] = acc[j] * f + v[j] * fi;
+        }
+      finish(r, mt, lt, acc);
+    }
+  } else {
     float mt = -INFINITY, lt = 0.f, acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.f;
-    if (x < rows) {
-      b = (int)(x / ((int64_t)p.T * p.n_head));
-      const int rem = (int)(x % ((int64_t)p.T * p.n_head));
-      t = rem / p.n_head, h = rem % p.n_head;
-      const int hk = h / a.rep, row = t * a.rep + h % a.rep, rt = row / MR, r = row % MR;
-      int64_t before = 0;
-      for (int i = 0; i < b; ++i) {
-        const TaSpan s = ta_span(p, i);
-        before += (s.hi - s.lo + BN - 1) / BN;
+    const int from = n * warp / WPR, to = nblk ? n * (warp + 1) / WPR : 0;
+    for (int c = from; c < to; c += 32) {
+      float mi = -INFINITY, li = 0.f;
+      int64_t base = 0;
+      if (c + lane < to) {
+        const int i = i0 + c + lane;
+        base = (int64_t)(2 * i + (i == i0 && ta_first_unit(total, runs, i) < s ? 1 : 0)) * MR + r0;
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + base * 2);
+        mi = ml.x, li = ml.y;
       }
-      sp = ta_span(p, b);
-      const int nblk = (sp.hi - sp.lo + BN - 1) / BN;
-      if (nblk == 0) {
-        const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
-        if (share == 0)
-          for (int d = lane; d < p.head_dim; d += 32) store_float(p.out, DT, oo + d, 0.f);
-        if (lane == 0 && (p.lens[b] < 0 || p.lens[b] > p.max_ctx)) raise_device_error(NS_DEVERR_ROUTE);
-      } else {
-        const int64_t s = (before * p.n_head_kv + (int64_t)hk * nblk) * a.row_tiles + (int64_t)rt * nblk, e = s + nblk;
-        const int i0 = (int)(((s + 1) * runs - 1) / total), i1 = (int)((e * runs - 1) / total);
-        cut = i0 != i1;  // else one run covered it
-        if (cut) {
-          const int n = i1 - i0 + 1, from = i0 + n * share / WPR, to = i0 + n * (share + 1) / WPR;
-          for (int c = from; c < to; c += 32) {
-            float mi = -INFINITY, li = 0.f;
-            int64_t base = 0;
-            if (c + lane < to) {
-              const int slot = 2 * (c + lane) + (ta_first_unit(total, runs, c + lane) >= s ? 0 : 1);
-              base = (int64_t)slot * MR + r;
-              const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + base * 2);
-              mi = ml.x, li = ml.y;
-            }
-            float mn = fmaxf(mt, mi);
+      float mn = fmaxf(mt, mi);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-            const float ref = mn == -INFINITY ? 0.f : mn;
-            const float f = ex2(mt - ref), fi = ex2(mi - ref);
-            mt = mn;
-            lt = lt * f + warp_sum(li * fi);
+      for (int o = 16; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float f = ex2(mt - ref), fi = ex2(mi - ref);
+      mt = mn;
+      lt = lt * f + warp_sum(li * fi);
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] *= f;
-            const int m = min(32, to - c);
-            for (int i = 0; i < m; i += 8) {
-              float v[8][V];
+      for (int j = 0; j < V; ++j) acc[j] *= f;
+      const int m = min(32, to - c);
+      for (int i = 0; i < m; i += 4) {  // four parts in flight; past the end the last one again, with weight zero
+        float v[4][V], w[4];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const int64_t at = __shfl_sync(0xffffffffu, base, (i + k) & 31);
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[k][j] = i + k < m ? a.part_o[at * HD + lane + 32 * j] : 0.f;
-              }
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float fk = __shfl_sync(0xffffffffu, fi, (i + k) & 31);
-#pragma unroll
-                for (int j = 0; j < V; ++j) acc[j] = i + k < m ? fmaf(v[k][j], fk, acc[j]) : acc[j];
-              }
-            }
-          }
+        for (int k = 0; k < 4; ++k) {
+          const int src = min(i + k, m - 1);
+          w[k] = __shfl_sync(0xffffffffu, fi, src);
+          if (i + k >= m) w[k] = 0.f;
+          load_part(__shfl_sync(0xffffffffu, base, src), v[k]);
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[j] = w[k] != 0.f ? fmaf(v[k][j], w[k], acc[j]) : acc[j];
       }
     }
-    if constexpr (WPR > 1) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) so[warp][lane + 32 * j] = acc[j];
-      if (lane == 0) sm[warp] = mt, sl[warp] = lt;
-      __syncthreads();
-      if (share == 0) {
-        float mn = -INFINITY;
+    for (int j = 0; j < V; ++j) so[warp][lane * V + j] = acc[j];
+    if (lane == 0) sm[warp] = mt, sl[warp] = lt;
+    __syncthreads();
+    if (warp == 0) {
+      mt = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < WPR; ++w) mn = fmaxf(mn, sm[warp + w]);
-        const float ref = mn == -INFINITY ? 0.f : mn;
-        lt = 0.f;
+      for (int w = 0; w < WPR; ++w) mt = fmaxf(mt, sm[w]);
+      const float ref = mt == -INFINITY ? 0.f : mt;
+      lt = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] = 0.f;
+      for (int j = 0; j < V; ++j) acc[j] = 0.f;
 #pragma unroll
-        for (int w = 0; w < WPR; ++w) {
-          const float f = ex2(sm[warp + w] - ref);
-          lt = fmaf(sl[warp + w], f, lt);
+      for (int w = 0; w < WPR; ++w) {
+        const float f = ex2(sm[w] - ref);
+        lt = fmaf(sl[w], f, lt);
 #pragma unroll
-          for (int j = 0; j < V; ++j) acc[j] = fmaf(so[warp + w][lane + 32 * j], f, acc[j]);
-        }
-        mt = mn;
+        for (int j = 0; j < V; ++j) acc[j] = f != 0.f ? fmaf(so[w][lane * V + j], f, acc[j]) : acc[j];
       }
+      finish(r0, mt, lt, acc);
     }
-    if (cut && share == 0) {
-      bool bad = false;
-      const bool used = p.parents ? tree_mask(t, [&](int i) { return p.parents[(int64_t)b * p.T + i]; }, &bad) != 0 : true;
-      const bool live = used && mt != -INFINITY && sp.len + t < p.max_ctx;
-      float scale = live ? 1.f / lt : 0.f;
-      if (live && p.sinks) {
-        const float sk = p.sinks[h] * 1.4426950408889634f, mm = fmaxf(mt, sk);
-        scale = ex2(mt - mm) / fmaf(lt, ex2(mt - mm), ex2(sk - mm));
-      }
-      const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (lane + 32 * j < p.head_dim) store_float(p.out, DT, oo + lane + 32 * j, live ? acc[j] * scale : 0.f);
-    }
-    if constexpr (WPR > 1) __syncthreads();
   }
+  if (lane == 0 && warp == 0 && r0 == 0 && (p.lens[b] < 0 || p.lens[b] > p.max_ctx)) raise_device_error(NS_DEVERR_ROUTE);
 }
 
 // ---- host
@@ -751,11 +789,14 @@ static int ta_groups(const ns_tree_attn_t* p) {  // WM: 16-row groups of a tile
 
 template <int DT, int HD>
 static int ta_join(const TaArgs& a, ns_stream_t stream) {
-  const int64_t rows = (int64_t)a.p.B * a.p.T * a.p.n_head;
-  if (rows <= 1024)  // few rows: their many parts are shared out among the warps
-    NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, kJoinWarps>, dim3((unsigned)rows), kJoinWarps * 32, 0, stream, 1, a));
+  const int64_t items = (int64_t)a.p.B * a.p.n_head_kv * a.row_tiles;
+  const int rows = std::min(a.tile_rows, a.p.T * a.rep);
+  if (items > INT32_MAX) return fail(NS_ERR_UNSUPPORTED, "ns_tree_attn: %lld tiles of rows", (long long)items);
+  if (items * rows <= 1024)  // few rows: their many parts are shared out among the warps
+    NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, kJoinWarps>, dim3((unsigned)items, rows), kJoinWarps * 32, 0, stream, 1, a));
   else
-    NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, 1>, dim3((unsigned)std::min<int64_t>((rows + 7) / 8, 1 << 20)),
+    NS_CUDA_TRY(launch_pdl(tree_attn_join_kernel<DT, HD, 1>,
+                           dim3((unsigned)items, (rows + kJoinWarps * kJoinRows - 1) / (kJoinWarps * kJoinRows)),
                            kJoinWarps * 32, 0, stream, 1, a));
   return NS_OK;
 }

@@ -113,6 +113,13 @@ __device__ __forceinline__ uint32_t seen_bits(int k0, int len, int klo, uint64_t
   return (uint32_t)below | (uint32_t)nodes;
 }
 
+// True in one lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
+
 struct TcAttnArgs {
   TaArgs a;
   CUtensorMap kmap, vmap;
@@ -166,7 +173,9 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
 
   // a wait that runs out ends this role; the others see the flag (or run out themselves)
   auto await = [&](uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
     if (*(volatile int*)&S.abort) return false;
     if (mbar_wait_bounded(bar, parity)) return true;
     *(volatile int*)&S.abort = 1;
@@ -437,54 +446,69 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
       return true;
     });
   } else if (warp == 8) {
-    // ------------------------------------------------------------------ products, one thread
-    if (lane == 0) {
-      int ck = 0, cv = 0, items = 0, steps[2] = {0, 0};
-      bool ok = true;
-      walk([&](const TcItem& it, int64_t) {
-        const int n_steps = PAIR ? 2 * it.n : it.n;
-        ok = await(&S.qready[0], items & 1) && (!PAIR || await(&S.qready[1], items & 1));
-        if (!ok) return false;
-        auto qk = [&](int k) {
-          const int s = k & 1, c = ck + (PAIR ? k >> 1 : k), st = c % NK;
-          if (!PAIR || s == 0)
-            if (!await(&S.kfull[st], (c / NK) & 1)) return false;
-          tc_fence_after();
-          const uint32_t qa = sq + (PAIR ? s : 0) * Cfg::kTile, ka = sk + st * Cfg::kTile;
+    // ------------------------------------------------------------------ products
+    // The whole warp walks and waits, one elected lane issues: operands stay warp-uniform, which the
+    // tensor instructions take from uniform registers.
+    // ring positions and phases of the next key block, the next value block and each slot's next step
+    int kst = 0, vst = 0, items = 0;
+    uint32_t kph = 0, vph = 0, pph[2] = {0, 0};
+    bool ok = true;
+    const uint64_t q0 = sw128_desc(sq, 16, 1024), kd = sw128_desc(sk, 16, 1024), vd = sw128_desc(sv, Cfg::kPanel, 1024);
+    walk([&](const TcItem& it, int64_t) {
+      const int n_steps = PAIR ? 2 * it.n : it.n;
+      ok = await_all(&S.qready[0], items & 1) && (!PAIR || await_all(&S.qready[1], items & 1));
+      if (!ok) return false;
+      auto qk = [&](int s) {
+        if (!PAIR || s == 0)
+          if (!await_all(&S.kfull[kst], kph)) return false;
+        tc_fence_after();
+        const uint64_t qa = q0 + (PAIR ? s : 0) * (Cfg::kTile >> 4), ka = kd + kst * (Cfg::kTile >> 4);
+        const uint32_t d = s_col(s);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * Cfg::kPanel + (kk & 3) * 32;
-            mma_f16_ss(s_col(s), sw128_desc(qa + off, 16, 1024), sw128_desc(ka + off, 16, 1024), idesc_f16<DT>(128, BN, false),
-                       kk > 0);
+            const uint32_t off = ((kk >> 2) * Cfg::kPanel + (kk & 3) * 32) >> 4;
+            mma_f16_ss(d, qa + off, ka + off, idesc_f16<DT>(128, BN, false), kk > 0);
           }
           tc_commit(&S.sfull[s]);
-          if (!PAIR || s == 1) tc_commit(&S.kempty[st]);
-          return true;
-        };
-        auto pv = [&](int k) {
-          const int s = k & 1, c = cv + (PAIR ? k >> 1 : k), st = c % NV;
-          if (!PAIR || s == 0)
-            if (!await(&S.vclean[st], (c / NV) & 1)) return false;
-          if (!await(&S.pready[s], steps[s] & 1)) return false;
-          ++steps[s];
-          tc_fence_after();
-          const uint32_t va = sv + st * Cfg::kTile;
+          if (!PAIR || s == 1) tc_commit(&S.kempty[kst]);
+        }
+        __syncwarp();
+        if (!PAIR || s == 1)
+          if (++kst == NK) kst = 0, kph ^= 1;
+        return true;
+      };
+      auto pv = [&](int s) {
+        if (!PAIR || s == 0)
+          if (!await_all(&S.vclean[vst], vph)) return false;
+        if (!await_all(&S.pready[s], pph[s])) return false;
+        pph[s] ^= 1;
+        tc_fence_after();
+        const uint64_t va = vd + vst * (Cfg::kTile >> 4);
+        const uint32_t d = o_col(s), pa = s_col(s);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk)
-            mma_f16_ts(o_col(s), s_col(s) + 8 * kk, sw128_desc(va + kk * 2048, Cfg::kPanel, 1024), idesc_f16<DT>(128, HD, true), 1);
+            mma_f16_ts(d, pa + 8 * kk, va + kk * (2048 >> 4), idesc_f16<DT>(128, HD, true), 1);
           tc_commit(&S.pvdone[s]);
-          if (!PAIR || s == 1) tc_commit(&S.vempty[st]);
-          return true;
-        };
-        ok = qk(0) && (n_steps < 2 || qk(1));
-        for (int k = 0; ok && k < n_steps; ++k) ok = pv(k) && (k + 2 >= n_steps || qk(k + 2));
-        ck += it.n, cv += it.n, ++items;
-        return ok;
-      });
-      if (!ok) {  // what was issued has to land before tensor memory is freed
-        tc_commit(&S.drain);
-        mbar_wait_bounded(&S.drain, 0);
+          if (!PAIR || s == 1) tc_commit(&S.vempty[vst]);
+        }
+        __syncwarp();
+        if (!PAIR || s == 1)
+          if (++vst == NV) vst = 0, vph ^= 1;
+        return true;
+      };
+      ok = qk(0) && (n_steps < 2 || qk(1));
+      for (int k = 0; ok && k < n_steps; k += 2) {
+        ok = pv(0) && (k + 2 >= n_steps || qk(0));
+        if (ok && k + 1 < n_steps) ok = pv(1) && (k + 3 >= n_steps || qk(1));
       }
+      ++items;
+      return ok;
+    });
+    if (!ok) {  // what was issued has to land before tensor memory is freed
+      if (elect_one()) tc_commit(&S.drain);
+      mbar_wait_bounded(&S.drain, 0);
     }
     __syncwarp();
   } else if (warp == 9) {
