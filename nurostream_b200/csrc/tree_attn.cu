@@ -19,6 +19,8 @@
 // products split each operand into two tf32 parts and add three mma.m16n8k8 (the product of the two
 // low parts, 2^-22 of the whole, is dropped), and the sum over a block joins the running output in
 // plain fp32 additions.
+#include <type_traits>
+
 #include "tree.cuh"
 
 namespace ns {
@@ -50,7 +52,7 @@ struct TaArgs {
 
 struct TaShared {
   uint64_t anc[kTreeMax];   // of the sequence at hand
-  int depth[kTreeMax];
+  int depth[kTreeMax], par[kTreeMax];
   int max_depth, bad_lo, bad_hi;
   uint32_t bad_keys[4];     // keys of the block whose values are not finite and not seen by all
   float wm[kTaWarps][16], wl[kTaWarps][16];
@@ -83,6 +85,18 @@ __device__ __forceinline__ int64_t ta_total(const TaArgs& a, int BN) {
     const TaSpan s = ta_span(a.p, b);
     n += (int64_t)((s.hi - s.lo + BN - 1) / BN);
   }
+  return n * a.p.n_head_kv * a.row_tiles;
+}
+
+// The same by a warp, a sequence per lane.
+__device__ __forceinline__ int64_t ta_total_warp(const TaArgs& a, int BN, int lane) {
+  int64_t n = 0;
+  for (int b = lane; b < a.p.B; b += 32) {
+    const TaSpan s = ta_span(a.p, b);
+    n += (int64_t)((s.hi - s.lo + BN - 1) / BN);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   return n * a.p.n_head_kv * a.row_tiles;
 }
 
@@ -162,6 +176,18 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Whether 16 bytes of shared memory hold a value that is not finite (an exponent of ones: adding one to
+// it carries into the sign's place, which the mask has cleared).
+template <int DT>
+__device__ __forceinline__ uint32_t not_finite(uint32_t saddr) {
+  uint32_t w[4];
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(saddr) : "memory");
+  constexpr uint32_t m = DT == NS_F32 ? 0x7F800000u : DT == NS_F16 ? 0x7C007C00u : 0x7F807F80u;
+  constexpr uint32_t one = DT == NS_F32 ? 0x00800000u : DT == NS_F16 ? 0x04000400u : 0x00800080u;
+  constexpr uint32_t top = DT == NS_F32 ? 0x80000000u : 0x80008000u;
+  return (((w[0] & m) + one) | ((w[1] & m) + one) | ((w[2] & m) + one) | ((w[3] & m) + one)) & top;
+}
+
 // 16-byte copy into shared memory, zeros when `ok` is false (nothing is read then).
 __device__ __forceinline__ void cp_async16_z(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
@@ -238,11 +264,11 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
       if (at.b != cur_b) {
         __syncthreads();
         if (tid == 0) S.max_depth = 0;
+        if (tid < p.T) S.par[tid] = p.parents ? p.parents[(int64_t)at.b * p.T + tid] : tid - 1;
         __syncthreads();
         if (tid < p.T) {
           bool bad = false;
-          uint64_t mk = p.parents ? tree_mask(tid, [&](int i) { return p.parents[(int64_t)at.b * p.T + i]; }, &bad)
-                                  : chain_mask(tid);
+          uint64_t mk = p.parents ? tree_mask(tid, [&](int i) { return S.par[i]; }, &bad) : chain_mask(tid);
           if (mk && sp.len + tid >= p.max_ctx) mk = 0, bad = true;
           if (bad) raise_device_error(NS_DEVERR_ROUTE);
           S.anc[tid] = mk;
@@ -313,25 +339,20 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
       // set to zero here and added, for the rows that see them, from the cache below
       if (tid < 4) S.bad_keys[tid] = 0;
       __syncthreads();
-      for (int c = tid; c < BN * CH; c += kTaThreads) {
-        const int r = c / CH;
-        const uint32_t ad = vs + r * RB + (c % CH) * 16;
-        bool bad = false;
+#pragma unroll 4
+      for (int i = 0; i < BN * CH / kTaThreads; ++i) {
+        const int c = tid + i * kTaThreads;
+        if (not_finite<DT>(vs + c * 16)) atomicOr(&S.bad_keys[c / CH >> 5], 1u << (c / CH & 31));
+      }
+      __syncthreads();
+      uint32_t any = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t w = lds32(ad + 4 * j);
-          if constexpr (DT == NS_F32) bad |= (w & 0x7F800000u) == 0x7F800000u;
-          else if constexpr (DT == NS_F16) bad |= (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
-          else bad |= (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
-        }
-        if (bad) atomicOr(&S.bad_keys[r >> 5], 1u << (r & 31));
+      for (int i = 0; i < BN / 32; ++i) any |= S.bad_keys[i];
+      if (any) {
+        for (int c = tid; c < BN * CH; c += kTaThreads)
+          if (S.bad_keys[c / CH >> 5] >> (c / CH & 31) & 1) sts128(vs + c * 16, 0, 0, 0, 0);
+        __syncthreads();
       }
-      __syncthreads();
-      for (int c = tid; c < BN * CH; c += kTaThreads) {
-        const int r = c / CH;
-        if (S.bad_keys[r >> 5] >> (r & 31) & 1) sts128(vs + r * RB + (c % CH) * 16, 0, 0, 0, 0);
-      }
-      __syncthreads();
     }
 
 #pragma unroll 1
@@ -562,7 +583,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) po[lane + 32 * i] = acc[i];
             if (lane == 0) {
-              a.part_ml[((int64_t)slot * MR + r) * 2] = mt;
+              a.part_ml[((int64_t)slot * MR + r) * 2] = S.anc[t] ? mt : -INFINITY;
               a.part_ml[((int64_t)slot * MR + r) * 2 + 1] = lt;
             }
           }
@@ -599,7 +620,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
             for (int n = 0; n < HD / 8; ++n)
               *reinterpret_cast<float2*>(po + n * 8 + 2 * tq) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
             if (tq == 0) {
-              a.part_ml[((int64_t)slot * MR + r) * 2] = m[i];
+              a.part_ml[((int64_t)slot * MR + r) * 2] = anc[i] ? m[i] : -INFINITY;
               a.part_ml[((int64_t)slot * MR + r) * 2 + 1] = l[i];
             }
           }
@@ -658,9 +679,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const _
 
   auto finish = [&](int r, float mt, float lt, float (&acc)[V]) {  // one row out
     const int row = rt * MR + r, t = row / a.rep, h = hk * a.rep + row % a.rep;
-    bool bad = false;
-    const bool used = p.parents ? tree_mask(t, [&](int i) { return p.parents[(int64_t)b * p.T + i]; }, &bad) != 0 : true;
-    const bool live = nblk && used && mt != -INFINITY && sp.len + t < p.max_ctx;
+    const bool live = mt != -INFINITY;  // an unused node's parts say -inf
     float scale = live ? 1.f / lt : 0.f;
     if (live && p.sinks) {
       const float sk = p.sinks[h] * 1.4426950408889634f, mm = fmaxf(mt, sk);
@@ -692,26 +711,38 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const _
   };
 
   if constexpr (WPR == 1) {
+    // the warp's rows side by side: their loads are in flight together
+    float mt[kJoinRows], lt[kJoinRows], acc[kJoinRows][V];
+#pragma unroll
+    for (int k = 0; k < kJoinRows; ++k) {
+      mt[k] = -INFINITY, lt[k] = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[k][j] = 0.f;
+    }
+    for (int i = 0; nblk && i < n; ++i) {
+      const int64_t at = (int64_t)(2 * (i0 + i) + (i == 0 && ta_first_unit(total, runs, i0) < s ? 1 : 0)) * MR;
+      float2 ml[kJoinRows];
+      float v[kJoinRows][V];
+#pragma unroll
+      for (int k = 0; k < kJoinRows; ++k) {
+        const int r = min(r0 + k * kJoinWarps + warp, n_rows - 1);
+        ml[k] = *reinterpret_cast<const float2*>(a.part_ml + (at + r) * 2);
+        load_part(at + r, v[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < kJoinRows; ++k) {
+        const float mn = fmaxf(mt[k], ml[k].x), ref = mn == -INFINITY ? 0.f : mn;
+        const float f = ex2(mt[k] - ref), fi = ex2(ml[k].x - ref);
+        mt[k] = mn;
+        lt[k] = lt[k] * f + ml[k].y * fi;
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[k][j] = acc[k][j] * f + v[k][j] * fi;
+      }
+    }
+#pragma unroll
     for (int k = 0; k < kJoinRows; ++k) {
       const int r = r0 + k * kJoinWarps + warp;
-      if (r >= n_rows) return;
-      float mt = -INFINITY, lt = 0.f, acc[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] = 0.f;
-      if (nblk)
-        for (int i = 0; i < n; ++i) {
-          const int64_t at = (int64_t)(2 * (i0 + i) + (i == 0 && ta_first_unit(total, runs, i0) < s ? 1 : 0)) * MR + r;
-          const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-          float v[V];
-          load_part(at, v);
-          const float mn = fmaxf(mt, ml.x), ref = mn == -INFINITY ? 0.f : mn;
-          const float f = ex2(mt - ref), fi = ex2(ml.x - ref);
-          mt = mn;
-          lt = lt * f + ml.y * fi;
-#pragma unroll
-          for (int j = 0; j < V; ++j) acc[j] = acc[j] * f + v[j] * fi;
-        }
-      finish(r, mt, lt, acc);
+      if (r < n_rows) finish(r, mt[k], lt[k], acc[k]);
     }
   } else {
     float mt = -INFINITY, lt = 0.f, acc[V];
@@ -809,7 +840,7 @@ static int ta_run(const ns_tree_attn_t* p, void* ws, ns_stream_t stream, size_t*
     *bytes = o_bytes + (size_t)2 * max_grid * MR * 2 * sizeof(float);
     return NS_OK;
   }
-  TaArgs a;
+  TaArgs a = {};
   a.p = *p;
   a.rep = p->n_head / p->n_head_kv;
   a.tile_rows = MR;

@@ -7,8 +7,8 @@
 // the same rows and take the blocks in turn, joined at the end.  Roles (one CTA an SM):
 //   warps 0-3, 4-7   softmax of slot 0 and 1, a row per thread: S from tensor memory, running maximum,
 //                    P = 2^(S - m) in 16 bits back over S, and the output at an item's end
-//   warp 8           issues the products: S = Q K^T (both operands in shared memory), O += P V (P in
-//                    tensor memory)
+//   warps 8, 11      issue the products of slot 0 and 1: S = Q K^T (both operands in shared memory),
+//                    O += P V (P in tensor memory)
 //   warp 9           TMA of key and value blocks into two rings
 //   warp 10          clears values that are not finite where a block is masked (see below)
 // The maximum that S is taken relative to is let lag: O is rescaled only when a row's maximum has
@@ -18,7 +18,7 @@
 // looks through the value tile of a masked block, zeroes such rows and leaves their bits for the softmax
 // warps, which add them, from the cache, to the rows that see them.
 
-constexpr int kTcAttnThreads = 384;  // warp 11 only fills its warpgroup
+constexpr int kTcAttnThreads = 384;
 constexpr int kTcAttnBlock = 128;  // keys
 constexpr float kTcAttnLag = 8.f;  // log2 of how far the maximum may lag
 
@@ -34,12 +34,14 @@ struct TcAttnCfg {
 struct TcAttnCtl {
   uint64_t kfull[4], kempty[4], vfull[4], vclean[4], vempty[4];
   uint64_t sfull[2], pready[2], pvdone[2], qready[2];
-  uint64_t meet, drain;
+  uint64_t meet, turn[2], drain[2];
+  int64_t u0, u1;              // the run, and where it starts
+  TaPos first;
   uint32_t tmem;
   int abort;
   uint32_t bad[4][4];          // value rows of a ring entry that are not finite
   uint64_t anc[kTreeMax];
-  int depth[kTreeMax];
+  int depth[kTreeMax], par[kTreeMax];
 };
 
 // K-major / MN-major operand in panels of 128-byte rows, 16-byte chunks XOR-swizzled by row % 8
@@ -105,6 +107,38 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tma
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar)) : "memory");
 }
 
+// Pairs of fp32 values in one 64-bit register pair.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// A starting value that the compiler does not see: it would clone a loop's body for its first turn, and
+// the launch would fetch the code of both (15 us more when the bodies are as long as the softmax's).
+__device__ __forceinline__ int opaque(int v) {
+  int r;
+  asm volatile("mov.u32 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 // Which of 32 keys from k0 on a row sees: cached ones from klo to len, then the nodes of vis.
 __device__ __forceinline__ uint32_t seen_bits(int k0, int len, int klo, uint64_t vis) {
   const int up = min(max(len - k0, 0), 32), dn = min(max(klo - k0, 0), 32), sh = k0 - len;
@@ -125,6 +159,10 @@ struct TcAttnArgs {
   CUtensorMap kmap, vmap;
 };
 
+// Polls of one wait, at most (some tenths of a second at the least): a plain count, so that the wait is a
+// few instructions and the loops of the roles stay in the instruction caches.
+constexpr int kTcAttnPolls = 1 << 24;
+
 // An item's part in this CTA's run: n blocks from block blk0.
 struct TcItem {
   TaPos pos;
@@ -144,28 +182,36 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
   const uint32_t sq = smem_addr(base), sk = sq + 2 * Cfg::kTile, sv = sk + NK * Cfg::kTile;
 
   if (tid == 0) {
+    constexpr int kUsers = PAIR ? 2 : 1;  // slots that use a ring entry
     prefetch_tmap(&args.kmap);
     prefetch_tmap(&args.vmap);
-    for (int i = 0; i < NK; ++i) mbar_init(&S.kfull[i], 1), mbar_init(&S.kempty[i], 1);
-    for (int i = 0; i < NV; ++i) mbar_init(&S.vfull[i], 1), mbar_init(&S.vclean[i], 1), mbar_init(&S.vempty[i], 1);
+    for (int i = 0; i < NK; ++i) mbar_init(&S.kfull[i], 1), mbar_init(&S.kempty[i], kUsers);
+    for (int i = 0; i < NV; ++i) mbar_init(&S.vfull[i], 1), mbar_init(&S.vclean[i], 1), mbar_init(&S.vempty[i], kUsers);
     for (int i = 0; i < 2; ++i)
-      mbar_init(&S.sfull[i], 1), mbar_init(&S.pready[i], 128), mbar_init(&S.pvdone[i], 1), mbar_init(&S.qready[i], 128);
-    mbar_init(&S.meet, 256);
-    mbar_init(&S.drain, 1);
+      mbar_init(&S.sfull[i], 1), mbar_init(&S.pready[i], 4), mbar_init(&S.pvdone[i], 1), mbar_init(&S.qready[i], 4);
+    mbar_init(&S.meet, 8);
+    for (int i = 0; i < 2; ++i) mbar_init(&S.turn[i], 1), mbar_init(&S.drain[i], 1);
     S.abort = 0;
     fence_mbar_init();
   }
   if (warp == 8) tmem_alloc(&S.tmem, 512);
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t total = ta_total(a, BN);
-  const int runs = ta_runs(a, total);
-  const bool busy = (int)blockIdx.x < runs;
-  const int64_t u0 = busy ? ta_first_unit(total, runs, blockIdx.x) : 0;
-  const int64_t u1 = busy ? ta_first_unit(total, runs, blockIdx.x + 1) : 0;
+  if (warp == 9) {  // the run
+    const int64_t total = ta_total_warp(a, BN, lane);
+    const int runs = ta_runs(a, total);
+    const bool busy = (int)blockIdx.x < runs;
+    const int64_t lo = busy ? ta_first_unit(total, runs, blockIdx.x) : 0;
+    if (lane == 0) {
+      S.u0 = lo;
+      S.u1 = busy ? ta_first_unit(total, runs, blockIdx.x + 1) : 0;
+      if (busy) S.first = ta_locate(a, BN, lo);
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  const int64_t u0 = S.u0, u1 = S.u1;
   const uint32_t tmem = S.tmem;
   // columns: S of slot 0, 1 at 0, 128 (P over them), O at 256, 256 + HD
   auto s_col = [&](int s) { return tmem + 128u * s; };
@@ -174,19 +220,35 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
   // a wait that runs out ends this role; the others see the flag (or run out themselves)
   auto await = [&](uint64_t* bar, uint32_t parity) {
 #pragma unroll 1
-    for (int i = 0; i < 64; ++i)
+    for (int i = 0; i < kTcAttnPolls; ++i) {
       if (mbar_try_wait(bar, parity)) return true;
-    if (*(volatile int*)&S.abort) return false;
-    if (mbar_wait_bounded(bar, parity)) return true;
+      if ((i & 1023) == 1023 && *(volatile int*)&S.abort) return false;
+    }
+    raise_device_error(NS_DEVERR_COPY_WAIT);
     *(volatile int*)&S.abort = 1;
     return false;
   };
-  // the same for a whole warp: either all of its threads go on or none
-  auto await_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, await(bar, parity)); };
+  // The same for a whole warp: all of its threads go on or none.  Every poll is voted on, so the loop never
+  // diverges: a vote after a loop that threads may leave apart costs 200 cycles even when all are ready.
+  auto await_all = [&](uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+    for (int i = 0; i < kTcAttnPolls; ++i) {
+      if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+      if ((i & 1023) == 1023 && __any_sync(0xffffffffu, *(volatile int*)&S.abort)) return false;
+    }
+    raise_device_error(NS_DEVERR_COPY_WAIT);
+    *(volatile int*)&S.abort = 1;
+    return false;
+  };
+  auto arrive_warp = [&](uint64_t* bar) {  // one arrival for what all of the warp's threads did
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
   // the items of the run, one after another
   auto walk = [&](auto&& body) {
     if (u0 >= u1) return;
-    TaPos at = ta_locate(a, BN, u0);
+    TaPos at = S.first;
+#pragma unroll 1
     for (int64_t u = u0; u < u1;) {
       const int n = (int)(u1 - u < at.nblk - at.blk ? u1 - u : at.nblk - at.blk);
       if (!body(TcItem{at, n}, u)) return;
@@ -201,38 +263,60 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
     return k0 + BN > sp.len || (p.window > 0 && sp.len + p.T - 1 - k0 >= p.window);
   };
 
-  // registers from the four helper warps to the softmax warps: 256 * 216 + 128 * 72 = 384 * 168
-  if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  // registers from the four helper warps to the softmax warps: 256 * 208 + 128 * 88 = 384 * 168
+  if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
 
   if (warp < 8) {
     // ------------------------------------------------------------------ softmax
     const int s = warp >> 2, row = tid & 127;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 * (warp % 4) in bits 16+
     const float sc = p.scale * 1.4426950408889634f;
-    int done = 0, vbase = 0, cur_b = -1;  // blocks of this slot, blocks of the run
+    int done = opaque(0), vbase = opaque(0), cur_b = opaque(-1);  // blocks of this slot, blocks of the run
     uint32_t met = 0;
     auto meet = [&]() {  // barrier of the two warpgroups; bounded like every wait
-      mbar_arrive(&S.meet);
+      arrive_warp(&S.meet);
       return await_all(&S.meet, met++ & 1);
     };
     walk([&](const TcItem& it, int64_t u) {
       const TaSpan sp = ta_span(p, it.pos.b);
       const int b = it.pos.b;
+      if (cur_b >= 0 && !meet()) return false;  // both slots are through with the last item
+      if (PAIR || s == 0) {  // this tile's queries, zeros past the rows and dims: a warp takes its 32 rows
+        constexpr int CH = HD / 8, RPI = 32 / CH;  // 16-byte chunks of a row, rows of one step
+        const int ch = lane % CH;
+        const uint32_t dst = sq + (PAIR ? s : 0) * Cfg::kTile + (ch >> 3) * Cfg::kPanel;
+        const uint16_t* qb = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] + ch * 8;
+#pragma unroll 8
+        for (int i = 0; i < 32 / RPI; ++i) {
+          const int rr = (warp & 3) * 32 + i * RPI + lane / CH, gr = it.pos.rt * MR + (PAIR ? s * 128 : 0) + rr;
+          const int qt = gr / a.rep;
+          const bool ok = qt < p.T && ch * 8 < p.head_dim;
+          const uint16_t* q = qb + (ok ? qt * p.q_stride[1] + (it.pos.h * a.rep + gr % a.rep) * p.q_stride[2] : 0);
+          const uint32_t d = dst + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
+          cp_async16_z(d, ok ? q : p.q, ok);
+        }
+        cp_async_commit();
+      }
       if (b != cur_b) {
-        if (!meet()) return false;
-        if (tid < p.T) {
-          bool bad = false;
-          uint64_t mk = p.parents ? tree_mask(tid, [&](int i) { return p.parents[(int64_t)b * p.T + i]; }, &bad)
-                                  : chain_mask(tid);
-          if (mk && sp.len + tid >= p.max_ctx) mk = 0, bad = true;
-          if (bad) raise_device_error(NS_DEVERR_ROUTE);
-          S.anc[tid] = mk;
-          S.depth[tid] = __popcll(mk) - 1;
+        if (warp == 0) {  // two nodes a lane, the parents in shared memory
+#pragma unroll
+          for (int i = 0; i < kTreeMax; i += 32)
+            if (i + lane < p.T) S.par[i + lane] = p.parents ? p.parents[(int64_t)b * p.T + i + lane] : i + lane - 1;
+          __syncwarp();
+#pragma unroll 1
+          for (int t = lane; t < p.T; t += 32) {
+            bool bad = false;
+            uint64_t mk = p.parents ? tree_mask(t, [&](int i) { return S.par[i]; }, &bad) : chain_mask(t);
+            if (mk && sp.len + t >= p.max_ctx) mk = 0, bad = true;
+            if (bad) raise_device_error(NS_DEVERR_ROUTE);
+            S.anc[t] = mk;
+            S.depth[t] = __popcll(mk) - 1;
+          }
         }
         cur_b = b;
+        if (!meet()) return false;  // the tree is there
       }
-      if (!meet()) return false;  // the tree is there; both slots are through with the last item's output
       const int r = it.pos.rt * MR + (PAIR ? s * 128 : 0) + row, t = r / a.rep;
       const int h = it.pos.h * a.rep + r % a.rep;
       const bool has_row = r < p.T * a.rep;
@@ -247,25 +331,6 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
           if (dep - S.depth[nd] >= p.window) vis &= ~(1ull << nd);
         }
       }
-      if (PAIR || s == 0) {  // this tile's queries, zeros past the rows and dims
-        const uint16_t* q = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2];
-        const uint32_t dst = sq + (PAIR ? s : 0) * Cfg::kTile + row * 128;
-        const bool vec = aligned16(q);
-#pragma unroll 4
-        for (int c = 0; c < HD / 8; ++c) {
-          uint32_t w[4] = {0, 0, 0, 0};
-          if (has_row && c * 8 < p.head_dim) {
-            if (vec) {
-              const uint4 x = *reinterpret_cast<const uint4*>(q + c * 8);
-              w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) w[j] = (uint32_t)q[c * 8 + 2 * j] | ((uint32_t)q[c * 8 + 2 * j + 1] << 16);
-            }
-          }
-          sts128(dst + (c >> 3) * Cfg::kPanel + (((c & 7) ^ (row & 7)) << 4), w[0], w[1], w[2], w[3]);
-        }
-      }
       {
         uint32_t z[32];
 #pragma unroll
@@ -274,34 +339,45 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
         for (int c = 0; c < HD / 32; ++c) tmem_st_x32(o_col(s) + lane_base + 32 * c, z);
         tmem_wait_st();
       }
+      cp_async_wait<0>();
       fence_proxy_async_smem();
       tc_fence_before();
-      if (PAIR || s == 0) mbar_arrive(&S.qready[PAIR ? s : 0]);
+      if (PAIR || s == 0) arrive_warp(&S.qready[PAIR ? s : 0]);
 
       float m = -INFINITY, l = 0.f;
+#pragma unroll 1
       for (int j = PAIR ? 0 : s; j < it.n; j += PAIR ? 1 : 2) {
         if (!await_all(&S.sfull[s], done & 1)) return false;
         tc_fence_after();
+        // The code of a block has to stay small: it is fetched anew by every launch and shares the
+        // instruction caches with the other roles.  So what is rare is a rolled loop over tensor memory.
+        const int k0 = sp.lo + (it.pos.blk + j) * BN;
+        const bool masked = is_masked(sp, k0);
+        if (masked) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float y[32];
+            tmem_ld_x32(s_col(s) + lane_base + 32 * c, y);
+            const uint32_t see = seen_bits(k0 + 32 * c, sp.len, klo, vis);
+            tmem_wait_ld_x32(y);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = see >> i & 1 ? y[i] : -INFINITY;
+            tmem_st_x32(s_col(s) + lane_base + 32 * c, reinterpret_cast<const uint32_t*>(y));
+          }
+          tmem_wait_st();
+        }
         float x[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_x32(s_col(s) + lane_base + 32 * c, x + 32 * c);
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_wait_ld_x32(x + 32 * c);
-        const int k0 = sp.lo + (it.pos.blk + j) * BN;
-        const bool masked = is_masked(sp, k0);
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t see = seen_bits(k0 + 32 * c, sp.len, klo, vis);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[32 * c + i] = see >> i & 1 ? x[32 * c + i] : -INFINITY;
-          }
-        }
         float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int i = 4; i < 128; i += 4)
+        for (int i = 4; i + 8 <= 128; i += 8)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], x[i + c]);
+          for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], x[i + c], x[i + 4 + c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], x[124 + c]);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
         // the reference of the exponentials: set by the first keys seen, moved when it lags too far
         const bool move = m == -INFINITY ? top != -INFINITY : top > m + kTcAttnLag;
@@ -323,22 +399,26 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
         }
         if (move) m = top;
         const float ref = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint64_t sum[2] = {0, 0};
+        const uint64_t sc2 = pair2(sc, sc), ref2 = pair2(-ref, -ref);
+        // probabilities, rounded to 16 bits: half an ulp each, as large as the output's own rounding
 #pragma unroll
-        for (int hf = 0; hf < 4; ++hf) {
+        for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int k = hf * 32 + 2 * i;
-            x[k] = ex2(fmaf(x[k], sc, -ref));
-            x[k + 1] = ex2(fmaf(x[k + 1], sc, -ref));
-            sum[i & 3] += x[k] + x[k + 1];
-            // rounded to 16 bits: half an ulp each, as large as the output's own rounding
-            pk[i] = pack16<DT>(x[k], x[k + 1]);
+            float e0, e1;
+            unpair2(fma2(pair2(x[32 * c + 2 * i], x[32 * c + 2 * i + 1]), sc2, ref2), e0, e1);
+            e0 = ex2(e0), e1 = ex2(e1);
+            sum[i & 1] = add2(sum[i & 1], pair2(e0, e1));
+            pk[i] = pack16<DT>(e0, e1);
           }
-          tmem_st_x16(s_col(s) + lane_base + 16 * hf, pk);
+          tmem_st_x16(s_col(s) + lane_base + 16 * c, pk);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float sum0, sum1, sum2, sum3;
+        unpair2(sum[0], sum0, sum1);
+        unpair2(sum[1], sum2, sum3);
+        l += (sum0 + sum1) + (sum2 + sum3);
         if (masked) {
           const int v = vbase + j, st = v % NV;
           if (!await_all(&S.vclean[st], (v / NV) & 1)) return false;
@@ -374,7 +454,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&S.pready[s]);
+        arrive_warp(&S.pready[s]);
         ++done;
       }
       vbase += it.n;
@@ -407,7 +487,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
       const int slot = 2 * blockIdx.x + (u - it.pos.blk <= u0 ? 0 : 1);
       const int64_t pr = (int64_t)slot * MR + (PAIR ? s * 128 : 0) + row;
       const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
-      if (!whole && has_row && (PAIR || s == 0)) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(m, l);
+      if (!whole && has_row && (PAIR || s == 0)) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(used ? m : -INFINITY, l);
       constexpr int NC = HD / 32;
 #pragma unroll 1
       for (int c = PAIR ? 0 : s * (NC / 2); c < (PAIR ? NC : (s + 1) * (NC / 2)); ++c) {
@@ -431,10 +511,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
               float y[8];
 #pragma unroll
               for (int k = 0; k < 8; ++k) y[k] = live ? o[i + k] * scale : 0.f;
-              if (aligned16(static_cast<uint16_t*>(p.out) + oo)) store_n<8>(p.out, DT, oo + 32 * c + i, y);
-              else
-#pragma unroll
-                for (int k = 0; k < 8; ++k) store_float(p.out, DT, oo + 32 * c + i + k, y[k]);
+              store_n<8>(p.out, DT, oo + 32 * c + i, y);
             }
         } else {
           float4* po = reinterpret_cast<float4*>(a.part_o + pr * HD + 32 * c);
@@ -445,70 +522,69 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
       tc_fence_before();
       return true;
     });
-  } else if (warp == 8) {
-    // ------------------------------------------------------------------ products
-    // The whole warp walks and waits, one elected lane issues: operands stay warp-uniform, which the
-    // tensor instructions take from uniform registers.
-    // ring positions and phases of the next key block, the next value block and each slot's next step
-    int kst = 0, vst = 0, items = 0;
-    uint32_t kph = 0, vph = 0, pph[2] = {0, 0};
+  } else if (warp == 8 || warp == 11) {
+    // ------------------------------------------------------------------ products of one slot
+    // A warp per slot, taking turns: P V of a block and Q K^T of the slot's next one go out together, then
+    // the other slot's.  In turns the slots stay half a period apart (issued side by side, both products
+    // finish late and both softmaxes then compete for the ex2 unit), and what a warp waits for is hidden
+    // behind the other's products.  The whole warp walks and waits, one elected lane issues, so the
+    // operands stay in uniform registers.
+    const int s = warp == 8 ? 0 : 1;
+    int cb = opaque(0), items = opaque(0), steps = opaque(0), turns = opaque(0);  // blocks of the run before this item, items, steps of this slot
     bool ok = true;
-    const uint64_t q0 = sw128_desc(sq, 16, 1024), kd = sw128_desc(sk, 16, 1024), vd = sw128_desc(sv, Cfg::kPanel, 1024);
+    const uint64_t qa = sw128_desc(sq + (PAIR ? s : 0) * Cfg::kTile, 16, 1024);
+    const uint64_t kd = sw128_desc(sk, 16, 1024), vd = sw128_desc(sv, Cfg::kPanel, 1024);
+    const uint32_t ds = s_col(s), dof = o_col(s);
     walk([&](const TcItem& it, int64_t) {
-      const int n_steps = PAIR ? 2 * it.n : it.n;
-      ok = await_all(&S.qready[0], items & 1) && (!PAIR || await_all(&S.qready[1], items & 1));
-      if (!ok) return false;
-      auto qk = [&](int s) {
-        if (!PAIR || s == 0)
-          if (!await_all(&S.kfull[kst], kph)) return false;
+      if (!(ok = await_all(&S.qready[PAIR ? s : 0], items & 1))) return false;
+      // one turn: P V of block c_pv (of the run; -1: none), Q K^T of block c_qk
+      auto issue = [&](int c_pv, int c_qk) {
+        const int vst = c_pv % NV, kst = c_qk % NK;
+        if (c_pv >= 0 && !await_all(&S.vclean[vst], (c_pv / NV) & 1)) return false;
+        if (c_qk >= 0 && !await_all(&S.kfull[kst], (c_qk / NK) & 1)) return false;
+        // slot 0's first turn is free, then each turn follows the other slot's last
+        if ((s == 1 || turns > 0) && !await_all(&S.turn[s], (turns - (s == 0 ? 1 : 0)) & 1)) return false;
+        ++turns;
+        if (c_pv >= 0 && !await_all(&S.pready[s], steps++ & 1)) return false;
         tc_fence_after();
-        const uint64_t qa = q0 + (PAIR ? s : 0) * (Cfg::kTile >> 4), ka = kd + kst * (Cfg::kTile >> 4);
-        const uint32_t d = s_col(s);
+        const uint64_t va = vd + vst * (Cfg::kTile >> 4), ka = kd + kst * (Cfg::kTile >> 4);
         if (elect_one()) {
+          if (c_pv >= 0) {
 #pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = ((kk >> 2) * Cfg::kPanel + (kk & 3) * 32) >> 4;
-            mma_f16_ss(d, qa + off, ka + off, idesc_f16<DT>(128, BN, false), kk > 0);
+            for (int kk = 0; kk < BN / 16; ++kk)
+              mma_f16_ts(dof, ds + 8 * kk, va + kk * (2048 >> 4), idesc_f16<DT>(128, HD, true), 1);
+            tc_commit(&S.pvdone[s]);
+            tc_commit(&S.vempty[vst]);
           }
-          tc_commit(&S.sfull[s]);
-          if (!PAIR || s == 1) tc_commit(&S.kempty[kst]);
-        }
-        __syncwarp();
-        if (!PAIR || s == 1)
-          if (++kst == NK) kst = 0, kph ^= 1;
-        return true;
-      };
-      auto pv = [&](int s) {
-        if (!PAIR || s == 0)
-          if (!await_all(&S.vclean[vst], vph)) return false;
-        if (!await_all(&S.pready[s], pph[s])) return false;
-        pph[s] ^= 1;
-        tc_fence_after();
-        const uint64_t va = vd + vst * (Cfg::kTile >> 4);
-        const uint32_t d = o_col(s), pa = s_col(s);
-        if (elect_one()) {
+          if (c_qk >= 0) {
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            mma_f16_ts(d, pa + 8 * kk, va + kk * (2048 >> 4), idesc_f16<DT>(128, HD, true), 1);
-          tc_commit(&S.pvdone[s]);
-          if (!PAIR || s == 1) tc_commit(&S.vempty[vst]);
+            for (int kk = 0; kk < HD / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * Cfg::kPanel + (kk & 3) * 32) >> 4;
+              mma_f16_ss(ds, qa + off, ka + off, idesc_f16<DT>(128, BN, false), kk > 0);
+            }
+            tc_commit(&S.sfull[s]);
+            tc_commit(&S.kempty[kst]);
+          }
+          mbar_arrive(&S.turn[s ^ 1]);
         }
         __syncwarp();
-        if (!PAIR || s == 1)
-          if (++vst == NV) vst = 0, vph ^= 1;
         return true;
       };
-      ok = qk(0) && (n_steps < 2 || qk(1));
-      for (int k = 0; ok && k < n_steps; k += 2) {
-        ok = pv(0) && (k + 2 >= n_steps || qk(0));
-        if (ok && k + 1 < n_steps) ok = pv(1) && (k + 3 >= n_steps || qk(1));
+      // both slots take the same number of turns; a slot without a block passes
+      constexpr int step = PAIR ? 1 : 2;
+      const int j0 = PAIR ? 0 : s, n_turns = PAIR ? it.n : (it.n + 1) / 2;
+      ok = issue(-1, j0 < it.n ? cb + j0 : -1);
+#pragma unroll 1
+      for (int k = 0; ok && k < n_turns; ++k) {
+        const int j = j0 + k * step;
+        ok = issue(j < it.n ? cb + j : -1, j + step < it.n ? cb + j + step : -1);
       }
-      ++items;
+      cb += it.n, ++items;
       return ok;
     });
     if (!ok) {  // what was issued has to land before tensor memory is freed
-      if (elect_one()) tc_commit(&S.drain);
-      mbar_wait_bounded(&S.drain, 0);
+      if (elect_one()) tc_commit(&S.drain[s]);
+      mbar_wait_bounded(&S.drain[s], 0);
     }
     __syncwarp();
   } else if (warp == 9) {
@@ -531,6 +607,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
           ++(key ? ck : cv);
           return true;
         };
+#pragma unroll 1
         for (int j = 0; ok && j < it.n; ++j) {
           ok = copy(true, j);
           if (PAIR) ok = ok && copy(false, j);
@@ -550,36 +627,36 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
     int cv = 0;
     walk([&](const TcItem& it, int64_t) {
       const TaSpan sp = ta_span(p, it.pos.b);
+#pragma unroll 1
       for (int j = 0; j < it.n; ++j, ++cv) {
         const int st = cv % NV;
-        if (!await(&S.vfull[st], (cv / NV) & 1)) return false;
+        if (!await_all(&S.vfull[st], (cv / NV) & 1)) return false;
         if (is_masked(sp, sp.lo + (it.pos.blk + j) * BN)) {
+          // a lane looks at one 16-byte chunk of one of four rows at a time; bit i: a bad row of group i
+          const uint32_t va = sv + st * Cfg::kTile;
+          uint32_t mine = 0;
+#pragma unroll 8
+          for (int i = 0; i < BN / 4; ++i) {
+            uint32_t acc = 0;
+#pragma unroll
+            for (int x = 0; x < Cfg::kPanels; ++x) acc |= not_finite<DT>(va + x * Cfg::kPanel + i * 512 + lane * 16);
+            mine |= acc ? 1u << i : 0u;
+          }
           if (lane < 4) S.bad[st][lane] = 0;
           __syncwarp();
-          const uint32_t va = sv + st * Cfg::kTile;
+          if (__any_sync(0xffffffffu, mine != 0)) {
 #pragma unroll 1
-          for (int rr = 0; rr < BN; rr += 4) {  // a lane looks through 16 bytes of one of four rows at a time
-            const int r = rr + (lane >> 3);
+            for (int i = 0; i < BN / 4; ++i)
+              if (mine >> i & 1) atomicOr(&S.bad[st][i >> 3], 1u << (4 * (i & 7) + (lane >> 3)));
+            __syncwarp();
+#pragma unroll 1
+            for (int i = 0; i < BN / 4; ++i)
+              if (S.bad[st][i >> 3] >> (4 * (i & 7) + (lane >> 3)) & 1)
 #pragma unroll
-            for (int x = 0; x < Cfg::kPanels; ++x) {
-              bool bad = false;
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const uint32_t v = lds32(va + x * Cfg::kPanel + r * 128 + (lane & 7) * 16 + 4 * w);
-                if constexpr (DT == NS_F16) bad |= (v & 0x7C00u) == 0x7C00u || (v & 0x7C000000u) == 0x7C000000u;
-                else bad |= (v & 0x7F80u) == 0x7F80u || (v & 0x7F800000u) == 0x7F800000u;
-              }
-              if (bad) atomicOr(&S.bad[st][r >> 5], 1u << (r & 31));
-            }
+                for (int x = 0; x < Cfg::kPanels; ++x) sts128(va + x * Cfg::kPanel + i * 512 + lane * 16, 0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
           }
-          __syncwarp();
-          for (int r = 0; r < BN; ++r)
-            if (S.bad[st][r >> 5] >> (r & 31) & 1)
-#pragma unroll
-              for (int x = 0; x < Cfg::kPanels; ++x)
-                if (lane < 8) sts128(va + x * Cfg::kPanel + r * 128 + lane * 16, 0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
         }
         if (lane == 0) mbar_arrive(&S.vclean[st]);
       }
@@ -592,10 +669,13 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
   if (warp == 8) tmem_dealloc(tmem, 512);
 }
 
-// Whether the tensor-core kernel takes a 16-bit call: many rows, and caches that a tensor map describes.
+// Whether the tensor-core kernel takes a 16-bit call: many rows, queries and outputs that start on 16
+// bytes, and caches that a tensor map describes.
 static bool ta_takes_tc(const ns_tree_attn_t* p) {
   const int rows = p->T * (p->n_head / p->n_head_kv);
   if (rows <= 32) return false;
+  if (!aligned_to(p->q, 16) || !aligned_to(p->out, 16) || !strides_multiple(p->q_stride, 3, 8) || !strides_multiple(p->o_stride, 3, 8))
+    return false;
   const int64_t dims[3] = {p->B, p->n_head_kv, p->max_ctx};
   for (int i = 0; i < 3; ++i)
     for (const int64_t* s : {p->kc_stride, p->vc_stride})
