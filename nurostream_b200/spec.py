@@ -21,11 +21,12 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from operator import attrgetter
 
 import torch
 
 from . import _lib
-from .fused import ns_dtype, stream_of
+from .fused import ns_dtype
 
 MAX_NODES = _lib.NS_TREE_MAX_NODES
 _I32, _F32 = torch.int32, torch.float32
@@ -49,6 +50,32 @@ def _dense(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, dev) ->
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
+
+
+# Argument checks and the parameter block that follows from shapes, strides, types and devices are worked out once
+# per such layout and kept by it: a call looks its layout up, copies the block and fills in the pointers.
+_LAYOUTS: dict = {}
+_MAX_LAYOUTS = 4096
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _sig(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _keep(key, layout):
+    if len(_LAYOUTS) >= _MAX_LAYOUTS:
+        _LAYOUTS.clear()
+    _LAYOUTS[key] = layout
+    return layout
+
+
+def _stream(dev: torch.device) -> int:
+    return _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
 
 
 def rope_tables(rotary_dim: int, n_pos: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
@@ -87,26 +114,57 @@ def rope_tables(rotary_dim: int, n_pos: int, base: float = 10000.0, scaling: str
     return (angle.cos() * amplitude).to(_F32).to(device), (angle.sin() * amplitude).to(_F32).to(device)
 
 
-def _rope_call(B, T, hq, hkv, hd, rotary_dim, interleaved, dtype, cache_dtype, max_ctx, lens, parents, positions, cos, sin,
-               q, k, v, q_out, kc, vc, dev) -> None:
+def _rope_layout(q, k, v, q_out, kc, vc, cos, sin, lens, parents, positions, rotary_dim, interleaved):
+    """Checks of a rope call (k, v and the caches may be None) and its parameter block without pointers."""
+    if q.dim() != 4 or (kc is not None and kc.dim() != 4):
+        raise ValueError("q must be (B, T, n_head, hd) and the caches (B, n_head_kv, max_ctx, hd)")
+    B, T, hq, hd = q.shape
+    hkv, max_ctx = (kc.shape[1], kc.shape[2]) if kc is not None else (0, 0)
+    dev, dt, cdt = q.device, q.dtype, q.dtype if kc is None else kc.dtype
+    if q_out.dtype != dt or (k is not None and (k.dtype != dt or v.dtype != dt)):
+        raise TypeError(f"q, k, v and q_out must have one type, got {[t.dtype for t in (q, k, v, q_out) if t is not None]}")
+    _rows("q", q, (B, T, hq, hd), dev)
+    _rows("q_out", q_out, (B, T, hq, hd), dev)
+    if kc is not None:
+        if vc.dtype != cdt:
+            raise TypeError(f"the caches must have one type, got {cdt} and {vc.dtype}")
+        _rows("k", k, (B, T, hkv, hd), dev)
+        _rows("v", v, (B, T, hkv, hd), dev)
+        _rows("k_cache", kc, (B, hkv, max_ctx, hd), dev)
+        _rows("v_cache", vc, (B, hkv, max_ctx, hd), dev)
     if cos.dtype != _F32 or sin.dtype != _F32 or cos.dim() != 2 or cos.shape != sin.shape or cos.stride() != sin.stride():
         raise TypeError("cos and sin must be fp32 tables (positions, at least rotary_dim / 2) of one layout")
     if cos.device != dev or sin.device != dev or (cos.stride(1) != 1 and cos.shape[1] > 1):
         raise ValueError(f"cos and sin must be on {dev} with contiguous rows")
-    if cos.shape[1] < rotary_dim // 2:
-        raise ValueError(f"tables of {cos.shape[1]} columns; rotary_dim {rotary_dim} needs {rotary_dim // 2}")
-    lens_p = _dense("lens", lens, _I32, (B,), dev)
-    par_p = None if parents is None else _dense("parents", parents, _I32, (B, T), dev)
-    pos_p = None if positions is None else _dense("positions", positions, _I32, (B, T), dev)
+    r = hd if rotary_dim is None else rotary_dim
+    if cos.shape[1] < r // 2:
+        raise ValueError(f"tables of {cos.shape[1]} columns; rotary_dim {r} needs {r // 2}")
+    _dense("lens", lens, _I32, (B,), dev)
+    for name, t in (("parents", parents), ("positions", positions)):
+        if t is not None:
+            _dense(name, t, _I32, (B, T), dev)
 
-    def ps(t):
-        return (None, _lib._S3()) if t is None else (t.data_ptr(), _lib._S3(*t.stride()[:3]))
+    def s3(t):
+        return _lib._S3() if t is None else _lib._S3(*t.stride()[:3])
 
-    (qp, qs), (kp, ks), (vp, vs), (op, os_), (kcp, kcs), (vcp, vcs) = map(ps, (q, k, v, q_out, kc, vc))
-    p = _lib.RopeAppendParams(B, T, hq, hkv, hd, rotary_dim, int(interleaved), dtype, cache_dtype, cos.shape[0], max_ctx,
-                              lens_p, par_p, pos_p, cos.data_ptr(), sin.data_ptr(), cos.stride(0), qp, kp, vp, op, kcp, vcp,
-                              qs, ks, vs, os_, kcs, vcs)
-    _lib.call("ns_rope_append", C.byref(p), torch.cuda.current_stream(dev).cuda_stream)
+    return bytes(_lib.RopeAppendParams(
+        B, T, hq, hkv, hd, r, int(interleaved), ns_dtype(dt), ns_dtype(cdt), cos.shape[0], max_ctx, None, None, None, None,
+        None, cos.stride(0), None, None, None, None, None, None, s3(q), s3(k), s3(v), s3(q_out), s3(kc), s3(vc)))
+
+
+def _rope_call(q, k, v, q_out, kc, vc, cos, sin, lens, parents, positions, rotary_dim, interleaved) -> None:
+    key = ("rope", _sig(q), _sig(k), _sig(v), _sig(q_out), _sig(kc), _sig(vc), _sig(cos), _sig(sin), _sig(lens),
+           _sig(parents), _sig(positions), rotary_dim, interleaved)
+    image = _LAYOUTS.get(key)
+    if image is None:
+        image = _keep(key, _rope_layout(q, k, v, q_out, kc, vc, cos, sin, lens, parents, positions, rotary_dim, interleaved))
+    p = _lib.RopeAppendParams.from_buffer_copy(image)
+    p.lens, p.parents, p.positions = lens.data_ptr(), _ptr(parents), _ptr(positions)
+    p.rope_cos, p.rope_sin = cos.data_ptr(), sin.data_ptr()
+    p.q, p.q_out = q.data_ptr(), q_out.data_ptr()
+    if kc is not None:
+        p.k, p.v, p.k_cache, p.v_cache = k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr()
+    _lib.call("ns_rope_append", C.byref(p), _stream(q.device))
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -123,24 +181,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     ``interleaved``.  q_out may be q (in place).  Rows of unused nodes: zero in q_out, nothing in the cache.
     With parents, T <= MAX_NODES; a chain (parents None) may have any T (a prompt).
     """
-    if q.dim() != 4 or k_cache.dim() != 4:
-        raise ValueError("q must be (B, T, n_head, hd) and the caches (B, n_head_kv, max_ctx, hd)")
-    B, T, hq, hd = q.shape
-    hkv, max_ctx = k_cache.shape[1], k_cache.shape[2]
-    dev, dt, cdt = q.device, q.dtype, k_cache.dtype
-    out = torch.empty((B, T, hq, hd), dtype=dt, device=dev) if q_out is None else q_out
-    if k.dtype != dt or v.dtype != dt or out.dtype != dt:
-        raise TypeError(f"q, k, v and q_out must have one type, got {dt}, {k.dtype}, {v.dtype}, {out.dtype}")
-    if v_cache.dtype != cdt:
-        raise TypeError(f"the caches must have one type, got {cdt} and {v_cache.dtype}")
-    _rows("q", q, (B, T, hq, hd), dev)
-    _rows("q_out", out, (B, T, hq, hd), dev)
-    _rows("k", k, (B, T, hkv, hd), dev)
-    _rows("v", v, (B, T, hkv, hd), dev)
-    _rows("k_cache", k_cache, (B, hkv, max_ctx, hd), dev)
-    _rows("v_cache", v_cache, (B, hkv, max_ctx, hd), dev)
-    _rope_call(B, T, hq, hkv, hd, hd if rotary_dim is None else rotary_dim, interleaved, ns_dtype(dt), ns_dtype(cdt),
-               max_ctx, lens, parents, positions, cos, sin, q, k, v, out, k_cache, v_cache, dev)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    _rope_call(q, k, v, out, k_cache, v_cache, cos, sin, lens, parents, positions, rotary_dim, interleaved)
     return out
 
 
@@ -149,17 +191,38 @@ def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch
     """x (B, T, heads, hd) rotated by the table rows of positions (B, T, int32); no cache.  out may be x."""
     if x.dim() != 4:
         raise ValueError("x must be (B, T, heads, hd)")
-    B, T, h, hd = x.shape
-    dev, dt = x.device, ns_dtype(x.dtype)
-    y = torch.empty((B, T, h, hd), dtype=x.dtype, device=dev) if out is None else out
-    if y.dtype != x.dtype:
-        raise TypeError(f"x and out must have one type, got {x.dtype} and {y.dtype}")
-    _rows("x", x, (B, T, h, hd), dev)
-    _rows("out", y, (B, T, h, hd), dev)
-    zero = torch.zeros(B, dtype=_I32, device=dev)
-    _rope_call(B, T, h, 0, hd, hd if rotary_dim is None else rotary_dim, interleaved, dt, dt, 0, zero, None, positions, cos,
-               sin, x, None, None, y, None, None, dev)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    zero = torch.zeros(x.shape[0], dtype=_I32, device=x.device)
+    _rope_call(x, None, None, y, None, None, cos, sin, zero, None, positions, rotary_dim, interleaved)
     return y
+
+
+def _attn_layout(q, kc, vc, o, lens, parents, sinks, window, scale):
+    """Checks of a tree_attention call, its parameter block without pointers, and its workspace bytes."""
+    if q.dim() != 4 or kc.dim() != 4:
+        raise ValueError("q must be (B, T, n_head, hd) and the caches (B, n_head_kv, max_ctx, hd)")
+    B, T, hq, hd = q.shape
+    hkv, max_ctx = kc.shape[1], kc.shape[2]
+    dev, dt = q.device, q.dtype
+    if kc.dtype != dt or vc.dtype != dt or o.dtype != dt:
+        raise TypeError(f"q, caches and out must have one type, got {dt}, {kc.dtype}, {vc.dtype}, {o.dtype}")
+    _rows("q", q, (B, T, hq, hd), dev)
+    _rows("out", o, (B, T, hq, hd), dev)
+    _rows("k_cache", kc, (B, hkv, max_ctx, hd), dev)
+    _rows("v_cache", vc, (B, hkv, max_ctx, hd), dev)
+    _dense("lens", lens, _I32, (B,), dev)
+    if parents is not None:
+        _dense("parents", parents, _I32, (B, T), dev)
+    if sinks is not None:
+        _dense("sinks", sinks, _F32, (hq,), dev)
+    s3 = _lib._S3
+    p = _lib.TreeAttnParams(
+        B, T, hq, hkv, hd, max_ctx, window, ns_dtype(dt), 1.0 / math.sqrt(hd) if scale is None else scale, None, None, None,
+        None, None, None, None, s3(*q.stride()[:3]), s3(*o.stride()[:3]), s3(*kc.stride()[:3]), s3(*vc.stride()[:3]))
+    n = C.c_size_t(0)
+    p.q = p.out = p.k_cache = p.v_cache = 256  # stand-ins: the size does not depend on them
+    _lib.call("ns_tree_attn_workspace_bytes", C.byref(p), C.byref(n))
+    return bytes(p), n.value
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lens: torch.Tensor,
@@ -172,30 +235,40 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     (T = 1: plain decode).  sinks: (n_head,) fp32 extra logits of the softmax.  window > 0: only positions above the
     node's own minus window.  scale: 1 / sqrt(hd) by default.  Returns (B, T, n_head, hd); zero rows for unused nodes.
     """
-    if q.dim() != 4 or k_cache.dim() != 4:
-        raise ValueError("q must be (B, T, n_head, hd) and the caches (B, n_head_kv, max_ctx, hd)")
-    B, T, hq, hd = q.shape
-    hkv, max_ctx = k_cache.shape[1], k_cache.shape[2]
-    dev, dt = q.device, q.dtype
-    o = torch.empty((B, T, hq, hd), dtype=dt, device=dev) if out is None else out
-    if k_cache.dtype != dt or v_cache.dtype != dt or o.dtype != dt:
-        raise TypeError(f"q, caches and out must have one type, got {dt}, {k_cache.dtype}, {v_cache.dtype}, {o.dtype}")
-    _rows("q", q, (B, T, hq, hd), dev)
-    _rows("out", o, (B, T, hq, hd), dev)
-    _rows("k_cache", k_cache, (B, hkv, max_ctx, hd), dev)
-    _rows("v_cache", v_cache, (B, hkv, max_ctx, hd), dev)
-    S3 = _lib._S3
-    p = _lib.TreeAttnParams(
-        B, T, hq, hkv, hd, max_ctx, window, ns_dtype(dt), 1.0 / math.sqrt(hd) if scale is None else scale,
-        _dense("lens", lens, _I32, (B,), dev), None if parents is None else _dense("parents", parents, _I32, (B, T), dev),
-        None if sinks is None else _dense("sinks", sinks, _F32, (hq,), dev), q.data_ptr(), k_cache.data_ptr(),
-        v_cache.data_ptr(), o.data_ptr(), S3(*q.stride()[:3]), S3(*o.stride()[:3]), S3(*k_cache.stride()[:3]),
-        S3(*v_cache.stride()[:3]))
-    n = C.c_size_t(0)
-    _lib.call("ns_tree_attn_workspace_bytes", C.byref(p), C.byref(n))
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-    _lib.call("ns_tree_attn", C.byref(p), ws.data_ptr(), n.value, torch.cuda.current_stream(dev).cuda_stream)
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    key = ("attn", _sig(q), _sig(k_cache), _sig(v_cache), _sig(o), _sig(lens), _sig(parents), _sig(sinks), window, scale)
+    layout = _LAYOUTS.get(key)
+    if layout is None:
+        layout = _keep(key, _attn_layout(q, k_cache, v_cache, o, lens, parents, sinks, window, scale))
+    image, ws_bytes = layout
+    p = _lib.TreeAttnParams.from_buffer_copy(image)
+    p.lens, p.parents, p.sinks = lens.data_ptr(), _ptr(parents), _ptr(sinks)
+    p.q, p.k_cache, p.v_cache, p.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr()
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    _lib.call("ns_tree_attn", C.byref(p), ws.data_ptr(), ws_bytes, _stream(q.device))
     return o
+
+
+def _verify_layout(tokens, logits, uniforms, race, parents, draft, temperature):
+    """Checks of a verify_tree call and its parameter block without pointers."""
+    if logits.dim() != 3 or tokens.dim() != 2:
+        raise ValueError("tokens must be (B, T) and logits (B, T, V)")
+    B, T, V = logits.shape
+    dev = logits.device
+    _rows("logits", logits, (B, T, V), dev)
+    if draft is not None:
+        _rows("draft_probs", draft, (B, T, V), dev)
+    _dense("tokens", tokens, _I32, (B, T), dev)
+    _dense("uniforms", uniforms, _F32, (B, T), dev)
+    _dense("race", race, _F32, (B, V), dev)
+    if parents is not None:
+        _dense("parents", parents, _I32, (B, T), dev)
+    if temperature is not None:
+        _dense("temperature", temperature, _F32, (B,), dev)
+    s2 = _lib._S2
+    return bytes(_lib.TreeVerifyParams(
+        B, T, V, ns_dtype(logits.dtype), 0 if draft is None else ns_dtype(draft.dtype), None, None, None, None, None, None,
+        None, s2(*logits.stride()[:2]), s2() if draft is None else s2(*draft.stride()[:2]), None, None, None))
 
 
 def verify_tree(tokens: torch.Tensor, logits: torch.Tensor, uniforms: torch.Tensor, race: torch.Tensor,
@@ -211,26 +284,43 @@ def verify_tree(tokens: torch.Tensor, logits: torch.Tensor, uniforms: torch.Tens
     that come out are distributed as the target's own.  path (B, T): accepted nodes from node 0 on, then -1;
     n_accepted (B) drafts; next_token (B), drawn as the largest r / race (-1 if a row's logits are all -inf).
     """
-    if logits.dim() != 3 or tokens.dim() != 2:
-        raise ValueError("tokens must be (B, T) and logits (B, T, V)")
-    B, T, V = logits.shape
-    dev = logits.device
-    _rows("logits", logits, (B, T, V), dev)
-    if draft_probs is not None:
-        _rows("draft_probs", draft_probs, (B, T, V), dev)
-    S2 = _lib._S2
-    res = torch.empty(B * (T + 2), dtype=_I32, device=dev)
-    path, n_acc, nxt = res[:B * T].view(B, T), res[B * T:B * (T + 1)], res[B * (T + 1):]
-    p = _lib.TreeVerifyParams(
-        B, T, V, ns_dtype(logits.dtype), 0 if draft_probs is None else ns_dtype(draft_probs.dtype),
-        _dense("tokens", tokens, _I32, (B, T), dev), None if parents is None else _dense("parents", parents, _I32, (B, T), dev),
-        logits.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(),
-        _dense("uniforms", uniforms, _F32, (B, T), dev), _dense("race", race, _F32, (B, V), dev),
-        None if temperature is None else _dense("temperature", temperature, _F32, (B,), dev),
-        S2(*logits.stride()[:2]), S2() if draft_probs is None else S2(*draft_probs.stride()[:2]),
-        path.data_ptr(), n_acc.data_ptr(), nxt.data_ptr())
-    _lib.call("ns_tree_verify", C.byref(p), stream_of(logits))
+    key = ("verify", _sig(tokens), _sig(logits), _sig(uniforms), _sig(race), _sig(parents), _sig(draft_probs),
+           _sig(temperature))
+    image = _LAYOUTS.get(key)
+    if image is None:
+        image = _keep(key, _verify_layout(tokens, logits, uniforms, race, parents, draft_probs, temperature))
+    B, T = tokens.shape
+    p = _lib.TreeVerifyParams.from_buffer_copy(image)
+    path = torch.empty((B, T), dtype=_I32, device=logits.device)
+    res = torch.empty((2, B), dtype=_I32, device=logits.device)
+    n_acc, nxt = res.unbind(0)
+    p.tokens, p.logits, p.uniforms, p.race = tokens.data_ptr(), logits.data_ptr(), uniforms.data_ptr(), race.data_ptr()
+    p.parents, p.draft_probs, p.temperature = _ptr(parents), _ptr(draft_probs), _ptr(temperature)
+    p.path, p.n_accepted, p.next_token = path.data_ptr(), n_acc.data_ptr(), nxt.data_ptr()
+    _lib.call("ns_tree_verify", C.byref(p), _stream(logits.device))
     return path, n_acc, nxt
+
+
+_META = attrgetter("shape", "dtype", "device")
+
+
+def _commit_layout(n_layer, k0, v0, lens, path, n_accepted, new_lens):
+    """Checks of a commit_path call's first layer and integers, and its parameter block without pointers."""
+    if not 1 <= n_layer <= _lib.NS_COMMIT_MAX_LAYERS:
+        raise ValueError(f"{n_layer} layers; 1 to {_lib.NS_COMMIT_MAX_LAYERS} a call")
+    if k0.dim() != 4:
+        raise ValueError("caches must be (B, n_head_kv, max_ctx, hd)")
+    B, hkv, max_ctx, hd = k0.shape
+    dev = k0.device
+    _rows("k_cache", k0, (B, hkv, max_ctx, hd), dev)
+    _rows("v_cache", v0, (B, hkv, max_ctx, hd), dev)
+    T = path.shape[1] if path.dim() == 2 else 0
+    _dense("lens", lens, _I32, (B,), dev)
+    _dense("path", path, _I32, (B, T), dev)
+    _dense("n_accepted", n_accepted, _I32, (B,), dev)
+    _dense("new_lens", new_lens, _I32, (B,), dev)
+    return bytes(_lib.PathCommitParams(n_layer, B, T, hkv, hd, max_ctx, ns_dtype(k0.dtype), None, None, None, None,
+                                       _lib._S3(*k0.stride()[:3]), _lib._S3(*v0.stride()[:3])))
 
 
 def commit_path(caches, lens: torch.Tensor, path: torch.Tensor, n_accepted: torch.Tensor, *,
@@ -241,28 +331,22 @@ def commit_path(caches, lens: torch.Tensor, path: torch.Tensor, n_accepted: torc
     one layout; path (B, T) and n_accepted (B) from ``verify_tree``.  Returns the new lengths,
     lens + 1 + n_accepted (written to ``new_lens`` when given; it may not be ``lens``).  One launch.
     """
-    caches = list(caches)
     if not caches:
         raise ValueError("caches is empty")
-    if len(caches) > _lib.NS_COMMIT_MAX_LAYERS:
-        raise ValueError(f"{len(caches)} layers; at most {_lib.NS_COMMIT_MAX_LAYERS} a call")
-    k0, v0 = caches[0]
-    if k0.dim() != 4:
-        raise ValueError("caches must be (B, n_head_kv, max_ctx, hd)")
-    shape, ks, vs, dt, dev = k0.shape, k0.stride(), v0.stride(), k0.dtype, k0.device
-    B, hkv, max_ctx, hd = shape
-    _rows("k_cache", k0, tuple(shape), dev)
-    _rows("v_cache", v0, tuple(shape), dev)
-    T = path.shape[1] if path.dim() == 2 else 0
+    ks, vs = zip(*caches)
+    k0, v0, n = ks[0], vs[0], len(ks)
     out = torch.empty_like(lens) if new_lens is None else new_lens
-    p = _lib.PathCommitParams(len(caches), B, T, hkv, hd, max_ctx, ns_dtype(dt), _dense("lens", lens, _I32, (B,), dev),
-                              _dense("path", path, _I32, (B, T), dev), _dense("n_accepted", n_accepted, _I32, (B,), dev),
-                              _dense("new_lens", out, _I32, (B,), dev), _lib._S3(*ks[:3]), _lib._S3(*vs[:3]))
-    kp, vp = p.k_cache, p.v_cache
-    for i, (k, v) in enumerate(caches):
-        if (k.shape != shape or v.shape != shape or k.stride() != ks or v.stride() != vs or k.dtype != dt or v.dtype != dt
-                or k.device != dev or v.device != dev):
-            raise ValueError(f"layer {i}: every layer's caches must have the shape, strides, type and device of the first's")
-        kp[i], vp[i] = k.data_ptr(), v.data_ptr()
-    _lib.call("ns_path_commit", C.byref(p), stream_of(k0))
+    key = ("commit", n, _sig(k0), _sig(v0), _sig(lens), _sig(path), _sig(n_accepted), _sig(out))
+    image = _LAYOUTS.get(key)
+    if image is None:
+        image = _keep(key, _commit_layout(n, k0, v0, lens, path, n_accepted, out))
+    stride = torch.Tensor.stride
+    if (list(map(_META, ks + vs)).count(_META(k0)) != 2 * n or list(map(stride, ks)).count(k0.stride()) != n
+            or list(map(stride, vs)).count(v0.stride()) != n):
+        raise ValueError("every layer's caches must have the shape, type and device of the first's, and its strides")
+    p = _lib.PathCommitParams.from_buffer_copy(image)
+    p.lens, p.path, p.n_accepted, p.new_lens = lens.data_ptr(), path.data_ptr(), n_accepted.data_ptr(), out.data_ptr()
+    ptr = torch.Tensor.data_ptr
+    p.k_cache[:n], p.v_cache[:n] = list(map(ptr, ks)), list(map(ptr, vs))
+    _lib.call("ns_path_commit", C.byref(p), _stream(k0.device))
     return out
