@@ -5,26 +5,49 @@
 //   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin
 // over the pairs of the first rotary_dim dims, the table row being the token's position.
 //
-// Pure traffic: q, k and v are read once and written once.  A thread owns one unit: U elements of
-// each half (16 bytes of a 16-bit type), or U elements of an interleaved, passed-through or value
-// row, so the partner of every element is in its registers.  U = 8 needs 16-byte aligned rows and
-// a rotation that divides into such units; U = 1 (a pair of elements) takes everything else.
+// Pure traffic: q, k and v are read once and written once; what costs beside it are index arithmetic and
+// the table.  A unit is two octets of a row, with 8 whole pairs in it where it rotates, so the partner of
+// every element is in the thread's registers.  A thread keeps one unit of the row and takes it through
+// the heads of one token: one table slice, one division, for all of them.  The heads' elements are read
+// before the token's position is known (length, then depth in the tree, then the table's row: each
+// waits for the one before).  Rows that do not divide into octets on 16 bytes go pair by pair.
 #include "tree.cuh"
 
 namespace ns {
 
 constexpr int kRopeThreads = 128;
 
-// N consecutive elements of type DT at element i, widened / rounded.  N = 8: 16-byte accesses.
-template <int DT, int N>
-__device__ __forceinline__ void load_n(const void* p, int64_t i, float (&x)[N]) {
-  if constexpr (N == 8 && DT == NS_F32) {
-    const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    const float4 a = f[0], b = f[1];
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else if constexpr (N == 8) {
-    const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+// Eight consecutive values rounded to type dt at element i, on 16 bytes.
+__device__ __forceinline__ void store8(void* p, int dt, int64_t i, const float (&x)[8]) {
+  if (dt == NS_F32) {
+    float4* f = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+    f[0] = make_float4(x[0], x[1], x[2], x[3]);
+    f[1] = make_float4(x[4], x[5], x[6], x[7]);
+    return;
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (dt == NS_F16) {
+      const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Eight values of type DT from their registers.
+template <int DT>
+__device__ __forceinline__ void widen8(const uint4* v, float (&x)[8]) {
+  if constexpr (DT == NS_F32) {
+    const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]);
+  } else {
+    const uint32_t w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (DT == NS_F16) {
@@ -34,76 +57,144 @@ __device__ __forceinline__ void load_n(const void* p, int64_t i, float (&x)[N]) 
         x[2 * j] = __uint_as_float(w[j] << 16), x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
       }
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = load_float(p, DT, i + j);
   }
 }
 
-template <int N>
-__device__ __forceinline__ void store_n(void* p, int dt, int64_t i, const float (&x)[N]) {
-  if constexpr (N == 8) {
-    if (dt == NS_F32) {
-      float4* f = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
-      f[0] = make_float4(x[0], x[1], x[2], x[3]);
-      f[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (dt == NS_F16) {
-          const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        } else {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-      }
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) store_float(p, dt, i + j, x[j]);
-  }
-}
-
-template <int DT, int U>
-__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const __grid_constant__ ns_rope_append_t p) {
+// Where token t of sequence b stands: its cache slot, its table row, and whether it is used at all.  The
+// whole warp calls it (the walk up the tree is shuffles: the warp holds the parents, two per lane).
+struct RopeAt {
+  int64_t slot, pos;
+  bool used;
+};
+__device__ __forceinline__ RopeAt rope_at_token(const ns_rope_append_t& p, int64_t tok, int b, int t) {
   const int lane = threadIdx.x & 31;
+  const int len = tree_len(p.lens, b, p.max_ctx);
+  int depth = t;
+  bool used = true, bad = len < 0;
+  if (p.parents) {
+    const int32_t* par = p.parents + (int64_t)b * p.T;
+    const int p0 = lane < p.T ? par[lane] : -2, p1 = lane + 32 < p.T ? par[lane + 32] : -2;
+    const uint64_t m = tree_mask(t, [&](int i) { return __shfl_sync(0xffffffffu, i < 32 ? p0 : p1, i & 31); }, &bad);
+    used = m != 0;
+    depth = __popcll(m) - 1;
+  }
+  RopeAt at;
+  at.slot = (int64_t)len + t;
+  if (used && at.slot >= p.max_ctx && (p.k || p.v)) bad = true;
+  at.pos = used ? (int64_t)len + depth : 0;
+  if (used && p.positions) at.pos = p.positions[tok];
+  if (used && (at.pos < 0 || at.pos >= p.n_pos)) bad = true;
+  if (bad) {
+    used = false;
+    if (threadIdx.x == 0 && blockIdx.x == 0) raise_device_error(NS_DEVERR_ROUTE);
+  }
+  at.used = used;
+  if (!used) at.pos = 0;
+  return at;
+}
+
+constexpr int kRopeRowThreads = 256;
+
+// NU: heads a thread reads side by side (gridDim.x > 1 shares a token's heads out when tokens are few)
+template <int DT, bool INTER, int NU>
+__global__ void __launch_bounds__(kRopeRowThreads) rope_rows_kernel(const __grid_constant__ ns_rope_append_t p) {
+  const int per = p.head_dim / 16, n_rot = p.rotary_dim / 16;  // units of a row, and the rotating ones
+  const int row0 = threadIdx.x / per, u = threadIdx.x % per, step = kRopeRowThreads / per;
+  const int nq = p.q ? p.n_head : 0, nk = p.k ? p.n_head_kv : 0, nv = p.v ? p.n_head_kv : 0, rows = nq + nk + nv;
+  const bool rotates = u < n_rot;
+  // first elements of the unit's octets
+  const int d0 = !rotates || INTER ? 16 * u : 8 * u, d1 = !rotates || INTER ? 16 * u + 8 : p.rotary_dim / 2 + 8 * u;
   griddep_wait();
   griddep_launch_dependents();
-  // units of one head: rotating ones (pairs or octets), then passed-through ones
-  const int half = p.rotary_dim / 2;
-  const int pair = U == 8 ? 8 : 2;  // elements of an interleaved unit
-  const int n_rot = p.interleaved ? p.rotary_dim / pair : half / U;
-  const int n_head_units = n_rot + (p.head_dim - p.rotary_dim) / U, n_val_units = p.head_dim / U;
+  for (int64_t tok = blockIdx.y; tok < (int64_t)p.B * p.T; tok += gridDim.y) {
+    const int b = (int)(tok / p.T), t = (int)(tok % p.T);
+    const int64_t qo = b * p.q_stride[0] + t * p.q_stride[1], ko = b * p.k_stride[0] + t * p.k_stride[1],
+                  vo = b * p.v_stride[0] + t * p.v_stride[1];
+    bool first = true;
+    RopeAt at{0, 0, false};
+    float c[8], s[8];
+    for (int r0 = row0 + blockIdx.x * step * NU; r0 - row0 < rows; r0 += step * NU * gridDim.x) {
+      uint4 raw[NU][DT == NS_F32 ? 4 : 2];
+#pragma unroll
+      for (int k = 0; k < NU; ++k) {
+        const int r = r0 + k * step;
+        if (row0 >= step || r >= rows) continue;
+        const void* src = r < nq ? p.q : r < nq + nk ? p.k : p.v;
+        const int64_t so = r < nq ? qo + r * p.q_stride[2] : r < nq + nk ? ko + (r - nq) * p.k_stride[2] : vo + (r - nq - nk) * p.v_stride[2];
+        if constexpr (DT == NS_F32) {
+          const float* f = static_cast<const float*>(src) + so;
+          raw[k][0] = *reinterpret_cast<const uint4*>(f + d0), raw[k][1] = *reinterpret_cast<const uint4*>(f + d0 + 4);
+          raw[k][2] = *reinterpret_cast<const uint4*>(f + d1), raw[k][3] = *reinterpret_cast<const uint4*>(f + d1 + 4);
+        } else {
+          const uint16_t* f = static_cast<const uint16_t*>(src) + so;
+          raw[k][0] = *reinterpret_cast<const uint4*>(f + d0), raw[k][1] = *reinterpret_cast<const uint4*>(f + d1);
+        }
+      }
+      if (first) {
+        first = false;
+        at = rope_at_token(p, tok, b, t);
+        if (rotates) {
+          const uint4* ct = reinterpret_cast<const uint4*>(p.rope_cos + at.pos * p.table_stride + 8 * u);
+          const uint4* st = reinterpret_cast<const uint4*>(p.rope_sin + at.pos * p.table_stride + 8 * u);
+          const uint4 cr[2] = {ct[0], ct[1]}, sr[2] = {st[0], st[1]};
+          widen8<NS_F32>(cr, c);
+          widen8<NS_F32>(sr, s);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < NU; ++k) {
+        const int r = r0 + k * step;
+        if (row0 >= step || r >= rows || (r >= nq && !at.used)) continue;
+        float x[8], y[8];
+        constexpr int H = DT == NS_F32 ? 2 : 1;
+        widen8<DT>(raw[k], x);
+        widen8<DT>(raw[k] + H, y);
+        if (rotates && r < nq + nk) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            // pair j: its members are x[j], y[j], or neighbours 2j, 2j + 1 of the sixteen
+            float& a = INTER ? (j < 4 ? x[2 * (j & 3)] : y[2 * (j & 3)]) : x[j];
+            float& d = INTER ? (j < 4 ? x[2 * (j & 3) + 1] : y[2 * (j & 3) + 1]) : y[j];
+            const float a0 = a, e0 = d;
+            a = a0 * c[j] - e0 * s[j];
+            d = e0 * c[j] + a0 * s[j];
+          }
+        }
+        void* dst;
+        int64_t dofs;
+        if (r < nq) {
+          if (!at.used)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = y[j] = 0.f;
+          dst = p.q_out, dofs = b * p.qo_stride[0] + t * p.qo_stride[1] + r * p.qo_stride[2];
+        } else if (r < nq + nk) {
+          dst = p.k_cache, dofs = b * p.kc_stride[0] + (r - nq) * p.kc_stride[1] + at.slot * p.kc_stride[2];
+        } else {
+          dst = p.v_cache, dofs = b * p.vc_stride[0] + (r - nq - nk) * p.vc_stride[1] + at.slot * p.vc_stride[2];
+        }
+        const int dt = r < nq ? DT : p.cache_dtype;
+        store8(dst, dt, dofs + d0, x);
+        store8(dst, dt, dofs + d1, y);
+      }
+    }
+  }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kRopeThreads) rope_pairs_kernel(const __grid_constant__ ns_rope_append_t p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  // units of one head: its pairs, then the elements passed through
+  const int half = p.rotary_dim / 2, n_rot = half;
+  const int n_head_units = n_rot + (p.head_dim - p.rotary_dim), n_val_units = p.head_dim;
   const int nq = p.q ? p.n_head * n_head_units : 0, nk = p.k ? p.n_head_kv * n_head_units : 0;
   const int nv = p.v ? p.n_head_kv * n_val_units : 0;
 
   for (int64_t tok = blockIdx.y; tok < (int64_t)p.B * p.T; tok += gridDim.y) {
     const int b = (int)(tok / p.T), t = (int)(tok % p.T);
-    const int len = tree_len(p.lens, b, p.max_ctx);
-    int depth = t;
-    bool used = true, bad = len < 0;
-    if (p.parents) {  // the warp holds the sequence's parents, two per lane; the walk is shuffles
-      const int32_t* par = p.parents + (int64_t)b * p.T;
-      const int p0 = lane < p.T ? par[lane] : -2, p1 = lane + 32 < p.T ? par[lane + 32] : -2;
-      const uint64_t m = tree_mask(t, [&](int i) {
-        const int lo = __shfl_sync(0xffffffffu, p0, i & 31), hi = __shfl_sync(0xffffffffu, p1, i & 31);
-        return i < 32 ? lo : hi;
-      }, &bad);
-      used = m != 0;
-      depth = __popcll(m) - 1;
-    }
-    const int64_t slot = (int64_t)len + t;
-    if (used && slot >= p.max_ctx && (p.k || p.v)) bad = true;
-    int64_t pos = used ? (int64_t)len + depth : 0;
-    if (used && p.positions) pos = p.positions[tok];
-    if (used && (pos < 0 || pos >= p.n_pos)) bad = true;
-    if (bad) {
-      used = false;
-      if (threadIdx.x == 0 && blockIdx.x == 0) raise_device_error(NS_DEVERR_ROUTE);
-    }
+    const RopeAt at = rope_at_token(p, tok, b, t);
+    const bool used = at.used;
+    const int64_t slot = at.slot, pos = at.pos;
     const float* cs = p.rope_cos + pos * p.table_stride;
     const float* sn = p.rope_sin + pos * p.table_stride;
 
@@ -128,63 +219,46 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const __grid_
       } else {
         const int h = (i - nq - nk) / n_val_units;
         u = (i - nq - nk) % n_val_units;
-        so = b * p.v_stride[0] + t * p.v_stride[1] + h * p.v_stride[2] + u * U;
-        dofs = b * p.vc_stride[0] + h * p.vc_stride[1] + slot * p.vc_stride[2] + u * U;
-        float x[U];
-        load_n<DT, U>(p.v, so, x);
-        store_n<U>(p.v_cache, p.cache_dtype, dofs, x);
+        so = b * p.v_stride[0] + t * p.v_stride[1] + h * p.v_stride[2] + u;
+        dofs = b * p.vc_stride[0] + h * p.vc_stride[1] + slot * p.vc_stride[2] + u;
+        store_float(p.v_cache, p.cache_dtype, dofs, load_float(p.v, DT, so));
         continue;
       }
       if (u >= n_rot) {  // passed through
-        const int d = p.rotary_dim + (u - n_rot) * U;
-        float x[U];
-        load_n<DT, U>(src, so + d, x);
-#pragma unroll
-        for (int j = 0; j < U; ++j) x[j] = used ? x[j] : 0.f;
-        store_n<U>(dst, dt, dofs + d, x);
-      } else if (p.interleaved) {
-        constexpr int N = U == 8 ? 8 : 2;
-        float x[N], c[N / 2], s[N / 2];
-        load_n<DT, N>(src, so + u * N, x);
-#pragma unroll
-        for (int j = 0; j < N / 2; ++j) c[j] = cs[u * (N / 2) + j], s[j] = sn[u * (N / 2) + j];
-#pragma unroll
-        for (int j = 0; j < N / 2; ++j) {
-          const float a = x[2 * j], d = x[2 * j + 1];
-          x[2 * j] = used ? a * c[j] - d * s[j] : 0.f;
-          x[2 * j + 1] = used ? d * c[j] + a * s[j] : 0.f;
-        }
-        store_n<N>(dst, dt, dofs + u * N, x);
-      } else {
-        float x[U], y[U], c[U], s[U];
-        load_n<DT, U>(src, so + u * U, x);
-        load_n<DT, U>(src, so + half + u * U, y);
-        load_n<NS_F32, U>(cs, u * U, c);
-        load_n<NS_F32, U>(sn, u * U, s);
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          const float a = x[j], d = y[j];
-          x[j] = used ? a * c[j] - d * s[j] : 0.f;
-          y[j] = used ? d * c[j] + a * s[j] : 0.f;
-        }
-        store_n<U>(dst, dt, dofs + u * U, x);
-        store_n<U>(dst, dt, dofs + half + u * U, y);
+        const int d = p.rotary_dim + (u - n_rot);
+        store_float(dst, dt, dofs + d, used ? load_float(src, DT, so + d) : 0.f);
+        continue;
       }
+      const int d0 = p.interleaved ? 2 * u : u, d1 = p.interleaved ? 2 * u + 1 : half + u;
+      const float x = load_float(src, DT, so + d0), y = load_float(src, DT, so + d1), c = cs[u], s = sn[u];
+      store_float(dst, dt, dofs + d0, used ? x * c - y * s : 0.f);
+      store_float(dst, dt, dofs + d1, used ? y * c + x * s : 0.f);
     }
   }
 }
 
 template <int DT>
 static cudaError_t rope_launch(const ns_rope_append_t& p, bool vec, ns_stream_t stream) {
-  const int U = vec ? 8 : 1;
-  const int n_rot = p.interleaved ? p.rotary_dim / (vec ? 8 : 2) : p.rotary_dim / 2 / U;
-  const int head_units = n_rot + (p.head_dim - p.rotary_dim) / U;
-  const int units = (p.q ? p.n_head * head_units : 0) + (p.k ? p.n_head_kv * head_units : 0) +
-                    (p.v ? p.n_head_kv * (p.head_dim / U) : 0);
   const int64_t tokens = (int64_t)p.B * p.T;
-  dim3 grid((unsigned)((units + kRopeThreads - 1) / kRopeThreads), (unsigned)std::min<int64_t>(tokens, 65535));
-  return vec ? launch_pdl(rope_append_kernel<DT, 8>, grid, kRopeThreads, 0, stream, 1, p)
-             : launch_pdl(rope_append_kernel<DT, 1>, grid, kRopeThreads, 0, stream, 1, p);
+  const unsigned gy = (unsigned)std::min<int64_t>(tokens, 65535);
+  const int rows = (p.q ? p.n_head : 0) + (p.k ? p.n_head_kv : 0) + (p.v ? p.n_head_kv : 0);
+  if (!vec) {
+    const int64_t units = (int64_t)((p.q ? p.n_head : 0) + (p.k ? p.n_head_kv : 0)) * (p.head_dim - p.rotary_dim / 2) +
+                          (int64_t)(p.v ? p.n_head_kv : 0) * p.head_dim;
+    return launch_pdl(rope_pairs_kernel<DT>, dim3((unsigned)((units + kRopeThreads - 1) / kRopeThreads), gy), kRopeThreads, 0,
+                      stream, 1, p);
+  }
+  const int step = kRopeRowThreads / (p.head_dim / 16), parts = (rows + step - 1) / step;
+  // few tokens: a block for every part of a token's heads; many: a block a token, four heads in flight a thread
+  if (tokens * parts <= 1024) {
+    const dim3 grid((unsigned)parts, gy);
+    return p.interleaved ? launch_pdl(rope_rows_kernel<DT, true, 1>, grid, kRopeRowThreads, 0, stream, 1, p)
+                         : launch_pdl(rope_rows_kernel<DT, false, 1>, grid, kRopeRowThreads, 0, stream, 1, p);
+  }
+  constexpr int NU = DT == NS_F32 ? 2 : 4;
+  const dim3 grid(1, gy);
+  return p.interleaved ? launch_pdl(rope_rows_kernel<DT, true, NU>, grid, kRopeRowThreads, 0, stream, 1, p)
+                       : launch_pdl(rope_rows_kernel<DT, false, NU>, grid, kRopeRowThreads, 0, stream, 1, p);
 }
 
 }  // namespace ns
@@ -209,9 +283,9 @@ extern "C" int ns_rope_append(const ns_rope_append_t* p, ns_stream_t stream) {
   if ((int64_t)(p->n_head + 2 * (int64_t)p->n_head_kv) * p->head_dim > (1 << 28))
     return fail(NS_ERR_UNSUPPORTED, "ns_rope_append: %d + 2 x %d heads of %d", p->n_head, p->n_head_kv, p->head_dim);
   if ((!p->q || !p->n_head) && ((!p->k && !p->v) || !p->n_head_kv)) return NS_OK;
-  // 16-byte units where every row starts on 16 bytes and the rotation divides into them
+  // octets where every row starts on 16 bytes and the row and its rotation are whole units
   const int64_t m = p->dtype == NS_F32 ? 4 : 8, mc = p->cache_dtype == NS_F32 ? 4 : 8;
-  bool vec = p->head_dim % 8 == 0 && p->rotary_dim % (p->interleaved ? 8 : 16) == 0 && p->table_stride % 4 == 0 &&
+  bool vec = p->head_dim % 16 == 0 && p->head_dim <= 16 * kRopeRowThreads && p->rotary_dim % 16 == 0 && p->table_stride % 4 == 0 &&
              aligned_to(p->rope_cos, 16) && aligned_to(p->rope_sin, 16);
   if (p->q)
     vec = vec && aligned_to(p->q, 16) && aligned_to(p->q_out, 16) && strides_multiple(p->q_stride, 3, m) &&

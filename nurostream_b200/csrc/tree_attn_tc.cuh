@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
               float y[8];
 #pragma unroll
               for (int k = 0; k < 8; ++k) y[k] = live ? o[i + k] * scale : 0.f;
-              store_n<8>(p.out, DT, oo + 32 * c + i, y);
+              store8(p.out, DT, oo + 32 * c + i, y);
             }
         } else {
           float4* po = reinterpret_cast<float4*>(a.part_o + pr * HD + 32 * c);
