@@ -23,7 +23,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC", "-shared", "-cudart", "shared",
-    "-Xptxas", "-v", "-split-compile", "0",
+    "-Xptxas", "-v",
 ]
 
 
