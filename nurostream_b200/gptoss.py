@@ -356,3 +356,76 @@ class GptOssDecoder:
         head = V * H * 2 + H * 4 + V * 4
         return {"experts+router": moe, "attention weights": attn, "kv": kv, "lm_head": head + H * 2,
                 "total": moe + attn + kv + head + H * 2}
+
+
+class SpecDecoder:
+    """Speculative decoding on a ``GptOssDecoder``: one step takes a drafted tree of up to ``n_nodes`` tokens
+    through the decoder's weights and KV cache, verifies it and keeps the accepted path.
+
+    Node 0 is the last token whose position is not cached yet (the prompt's last, or the previous step's
+    ``next_token``); the others are drafts of the tokens after it, by whatever drafts (a small model, a
+    lookup in the text so far).  Per layer: the decoder's q/k/v projection of every node, ``spec.rope_append``,
+    ``spec.tree_attention``, the output projection, and the MoE layer over all nodes (``prefill_grouped``);
+    then the LM head, ``spec.verify_tree`` and ``spec.commit_path``.  The context length lives in
+    ``self.lens`` on the device and advances by the accepted nodes; plain ``decoder.step`` calls may follow at
+    that position.  One rank (world 1); a chain (parents None) or a tree of at most ``spec.MAX_NODES`` nodes.
+    """
+
+    def __init__(self, decoder: GptOssDecoder, n_nodes: int):
+        from . import spec
+        if decoder.world != 1:
+            raise ValueError("SpecDecoder runs on one rank")
+        if not 1 <= n_nodes <= spec.MAX_NODES:
+            raise ValueError(f"n_nodes {n_nodes} outside 1..{spec.MAX_NODES}")
+        self.dec, self.n_nodes, self._spec = decoder, n_nodes, spec
+        sh, dev, T = decoder.shape, decoder.device, n_nodes
+        f32 = dict(dtype=torch.float32, device=dev)
+        self.lens = torch.full((1,), decoder.ctx, dtype=torch.int32, device=dev)
+        self.tokens = torch.zeros((1, T), dtype=torch.int32, device=dev)
+        self.xs = [torch.empty((T, sh.n_embd), **f32) for _ in range(3)]
+        self.qkv = torch.empty((T, sh.q_dim + 2 * sh.kv_dim), **f32)
+        self.q = torch.empty((1, T, sh.n_head, sh.head_dim), **f32)
+        self.attn_out = torch.empty((1, T, sh.n_head, sh.head_dim), **f32)
+        self.logits = torch.empty((1, T, sh.vocab_size), **f32)
+        self.caches = [(a.k_cache[None], a.v_cache[None]) for a in decoder.attn]
+
+    def forward(self, tokens: torch.Tensor, parents: torch.Tensor | None = None) -> torch.Tensor:
+        """The target's logits (1, T, V) after every node; keys and values go to slots lens..lens + T - 1."""
+        spec, dec, T = self._spec, self.dec, self.n_nodes
+        sh, stream = dec.shape, torch.cuda.current_stream(dec.device).cuda_stream
+        self.tokens.copy_(tokens.view(1, T))
+        x, xa, nxt = self.xs
+        for t in range(T):
+            _lib.call("ns_embed", dec.embd.data_ptr(), _lib.NS_BF16, sh.vocab_size, sh.n_embd,
+                      self.tokens.data_ptr() + 4 * t, x[t].data_ptr(), stream)
+        q, k, v = self.qkv.view(1, T, sh.n_head + 2 * sh.n_head_kv, sh.head_dim).split(
+            [sh.n_head, sh.n_head_kv, sh.n_head_kv], dim=2)
+        for l, layer in enumerate(dec.attn):
+            for t in range(T):
+                _lib.call("ns_dense_gemv", C.byref(layer.qkv_params(x[t], self.qkv[t])), stream)
+            kc, vc = self.caches[l]
+            spec.rope_append(q, k, v, dec.rope_cos, dec.rope_sin, kc, vc, self.lens, parents, q_out=self.q)
+            spec.tree_attention(self.q, kc, vc, self.lens, parents, sinks=layer.sinks, window=layer.window,
+                                out=self.attn_out)
+            for t in range(T):
+                _lib.call("ns_dense_gemv", C.byref(layer.oproj_params(self.attn_out[0, t], x[t], xa[t])), stream)
+            if T == 1:
+                dec.moe[l](xa, out=nxt)
+            else:
+                dec.moe[l].prefill_grouped(xa, out=nxt)
+            x, nxt = nxt, x
+        head = _lib.DenseGemvParams.from_buffer_copy(dec._head)
+        for t in range(T):
+            head.x, head.seg[0].y = x[t].data_ptr(), self.logits[0, t].data_ptr()
+            _lib.call("ns_dense_gemv", C.byref(head), stream)
+        return self.logits
+
+    def step(self, tokens: torch.Tensor, uniforms: torch.Tensor, race: torch.Tensor, parents: torch.Tensor | None = None,
+             draft_probs: torch.Tensor | None = None, temperature: torch.Tensor | None = None):
+        """One speculative step: (path, n_accepted, next_token) as ``spec.verify_tree`` gives them, the accepted
+        nodes' keys and values in place and ``self.lens`` advanced past them.  No host synchronisation."""
+        logits = self.forward(tokens, parents)
+        path, n_acc, token = self._spec.verify_tree(self.tokens, logits, uniforms, race, parents, draft_probs=draft_probs,
+                                                    temperature=temperature)
+        self.lens = self._spec.commit_path(self.caches, self.lens, path, n_acc)
+        return path, n_acc, token

@@ -1,0 +1,90 @@
+"""SpecDecoder: a drafted tree through a whole GPT-OSS model gives what decoding token by token gives."""
+import pytest
+import torch
+
+from nurostream_b200 import _lib
+from nurostream_b200.gptoss import GptOssDecoder, SpecDecoder
+from nurostream_b200.shapes import GptOssShape
+
+pytestmark = pytest.mark.gpu
+
+SHAPE = dict(n_layer=3, n_embd=256, n_head=8, n_head_kv=2, head_dim=64, n_ffn=256, vocab_size=512, n_expert=8,
+             n_expert_used=2, n_ffn_expert=256, sliding_window=24)
+CTX = 40
+
+
+def _decoder():
+    return GptOssDecoder(GptOssShape(**SHAPE), torch.device("cuda", 0), seed=3, ctx=CTX, max_ctx=128)
+
+
+def _greedy(n, first=5):
+    """Tokens and logits of n plain decode steps from token `first` at position CTX."""
+    dec, toks, rows = _decoder(), [first], []
+    for i in range(n):
+        dec.set_token(toks[-1], CTX + i)
+        rows.append(dec.step().clone())
+        toks.append(int(rows[-1].argmax()))
+    return toks, rows
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _close(a, b):
+    # the same fp32 arithmetic with other summation orders, over three layers; the suite's layer tests hold 2e-5 each
+    assert (a - b).abs().max() <= 1e-4 * b.abs().max()
+
+
+def test_chain_of_right_drafts_is_accepted_whole():
+    toks, rows = _greedy(7)
+    s = SpecDecoder(_decoder(), 6)
+    u, race = torch.rand(1, 6, device="cuda"), torch.ones(1, 512, device="cuda")
+    path, n, nxt = s.step(_ints(toks[:6]), u, race, temperature=torch.zeros(1, device="cuda"))
+    assert path.tolist() == [list(range(6))] and int(n) == 5 and int(nxt) == toks[6] and int(s.lens) == CTX + 6
+    for t in range(6):
+        _close(s.logits[0, t], rows[t])
+    s.dec.set_token(int(nxt), int(s.lens))        # plain decoding goes on from the advanced cache
+    _close(s.dec.step(), rows[6])
+    assert _lib.device_error() == 0
+
+
+def test_tree_keeps_the_right_branch_only():
+    toks, rows = _greedy(9)
+    bad = [(t + 7) % 512 for t in toks]
+    #        0        1       2        3       4        5       6        7
+    tokens = [toks[0], bad[1], toks[1], bad[2], toks[2], bad[3], toks[3], bad[4]]
+    parents = [-1, 0, 0, 1, 2, 2, 4, 6]
+    s = SpecDecoder(_decoder(), 8)
+    u, race = torch.rand(1, 8, device="cuda"), torch.ones(1, 512, device="cuda")
+    greedy = torch.zeros(1, device="cuda")
+    path, n, nxt = s.step(_ints(tokens), u, race, _ints([parents]), temperature=greedy)
+    assert path[0, :4].tolist() == [0, 2, 4, 6] and int(n) == 3 and int(nxt) == toks[4] and int(s.lens) == CTX + 4
+    for node, row in ((0, 0), (2, 1), (4, 2), (6, 3)):
+        _close(s.logits[0, node], rows[row])
+    # a second step over the moved cache, then a plain one
+    tokens = [toks[4], toks[5], toks[6], bad[7], 0, 0, 0, 0]
+    path, n, nxt = s.step(_ints(tokens), u, race, _ints([[-1, 0, 1, 2, -2, -2, -2, -2]]), temperature=greedy)
+    assert path[0, :4].tolist() == [0, 1, 2, -1] and int(n) == 2 and int(nxt) == toks[7] and int(s.lens) == CTX + 7
+    for t in range(3):
+        _close(s.logits[0, t], rows[4 + t])
+    s.dec.set_token(int(nxt), int(s.lens))
+    _close(s.dec.step(), rows[7])
+    assert _lib.device_error() == 0
+
+
+def test_one_node_is_a_plain_step():
+    toks, rows = _greedy(3)
+    s = SpecDecoder(_decoder(), 1)
+    u, race = torch.rand(1, 1, device="cuda"), torch.ones(1, 512, device="cuda")
+    for i in range(3):
+        _, n, nxt = s.step(_ints([toks[i]]), u, race, temperature=torch.zeros(1, device="cuda"))
+        _close(s.logits[0, 0], rows[i])
+        assert int(n) == 0 and int(nxt) == toks[i + 1] and int(s.lens) == CTX + i + 1
+
+
+def test_refusals():
+    dec = _decoder()
+    for n in (0, 65):
+        with pytest.raises(ValueError):
+            SpecDecoder(dec, n)
