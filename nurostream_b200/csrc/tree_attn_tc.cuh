@@ -159,9 +159,9 @@ struct TcAttnArgs {
   CUtensorMap kmap, vmap;
 };
 
-// Polls of one wait, at most (some tenths of a second at the least): a plain count, so that the wait is a
-// few instructions and the loops of the roles stay in the instruction caches.
-constexpr int kTcAttnPolls = 1 << 24;
+// A wait looks at the clock and at the other roles only every so many polls: the loops of the roles have
+// to stay in the instruction caches.
+constexpr uint32_t kTcAttnPolls = 1024;
 
 // An item's part in this CTA's run: n blocks from block blk0.
 struct TcItem {
@@ -217,28 +217,33 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
   auto s_col = [&](int s) { return tmem + 128u * s; };
   auto o_col = [&](int s) { return tmem + 256u + (uint32_t)HD * s; };
 
-  // a wait that runs out ends this role; the others see the flag (or run out themselves)
-  auto await = [&](uint64_t* bar, uint32_t parity) {
-#pragma unroll 1
-    for (int i = 0; i < kTcAttnPolls; ++i) {
-      if (mbar_try_wait(bar, parity)) return true;
-      if ((i & 1023) == 1023 && *(volatile int*)&S.abort) return false;
+  // A wait that runs out (kWaitLimitNs) ends this role; the others see the flag, or run out themselves.
+  auto give_up = [&](uint64_t& since) {
+    const uint64_t now = globaltimer_ns();
+    if (since == 0) since = now;
+    if (now - since > kWaitLimitNs) {
+      raise_device_error(NS_DEVERR_COPY_WAIT);
+      *(volatile int*)&S.abort = 1;
     }
-    raise_device_error(NS_DEVERR_COPY_WAIT);
-    *(volatile int*)&S.abort = 1;
-    return false;
+    return *(volatile int*)&S.abort != 0;
+  };
+  auto await = [&](uint64_t* bar, uint32_t parity) {
+    uint64_t since = 0;
+#pragma unroll 1
+    for (uint32_t i = 1;; ++i) {
+      if (mbar_try_wait(bar, parity)) return true;
+      if (i % kTcAttnPolls == 0 && give_up(since)) return false;
+    }
   };
   // The same for a whole warp: all of its threads go on or none.  Every poll is voted on, so the loop never
   // diverges: a vote after a loop that threads may leave apart costs 200 cycles even when all are ready.
   auto await_all = [&](uint64_t* bar, uint32_t parity) {
+    uint64_t since = 0;
 #pragma unroll 1
-    for (int i = 0; i < kTcAttnPolls; ++i) {
+    for (uint32_t i = 1;; ++i) {
       if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-      if ((i & 1023) == 1023 && __any_sync(0xffffffffu, *(volatile int*)&S.abort)) return false;
+      if (i % kTcAttnPolls == 0 && __any_sync(0xffffffffu, give_up(since))) return false;
     }
-    raise_device_error(NS_DEVERR_COPY_WAIT);
-    *(volatile int*)&S.abort = 1;
-    return false;
   };
   auto arrive_warp = [&](uint64_t* bar) {  // one arrival for what all of the warp's threads did
     __syncwarp();
@@ -287,14 +292,28 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
         const int ch = lane % CH;
         const uint32_t dst = sq + (PAIR ? s : 0) * Cfg::kTile + (ch >> 3) * Cfg::kPanel;
         const uint16_t* qb = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] + ch * 8;
-#pragma unroll 8
-        for (int i = 0; i < 32 / RPI; ++i) {
+        auto chunk = [&](int i, auto&& put) {
           const int rr = (warp & 3) * 32 + i * RPI + lane / CH, gr = it.pos.rt * MR + (PAIR ? s * 128 : 0) + rr;
           const int qt = gr / a.rep;
           const bool ok = qt < p.T && ch * 8 < p.head_dim;
           const uint16_t* q = qb + (ok ? qt * p.q_stride[1] + (it.pos.h * a.rep + gr % a.rep) * p.q_stride[2] : 0);
           const uint32_t d = dst + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
-          cp_async16_z(d, ok ? q : p.q, ok);
+          put(d, q, ok);
+        };
+        if (a.vec & 1) {
+#pragma unroll 8
+          for (int i = 0; i < 32 / RPI; ++i)
+            chunk(i, [&](uint32_t d, const uint16_t* q, bool ok) { cp_async16_z(d, ok ? (const void*)q : p.q, ok); });
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < 32 / RPI; ++i)
+            chunk(i, [&](uint32_t d, const uint16_t* q, bool ok) {
+              uint32_t w[4] = {0, 0, 0, 0};
+              if (ok)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (uint32_t)q[2 * j] | ((uint32_t)q[2 * j + 1] << 16);
+              sts128(d, w[0], w[1], w[2], w[3]);
+            });
         }
         cp_async_commit();
       }
@@ -511,7 +530,12 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
               float y[8];
 #pragma unroll
               for (int k = 0; k < 8; ++k) y[k] = live ? o[i + k] * scale : 0.f;
-              store8(p.out, DT, oo + 32 * c + i, y);
+              if (a.vec & 2) {
+                store8(p.out, DT, oo + 32 * c + i, y);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) store_float(p.out, DT, oo + 32 * c + i + k, y[k]);
+              }
             }
         } else {
           float4* po = reinterpret_cast<float4*>(a.part_o + pr * HD + 32 * c);
@@ -669,13 +693,14 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
   if (warp == 8) tmem_dealloc(tmem, 512);
 }
 
-// Whether the tensor-core kernel takes a 16-bit call: many rows, queries and outputs that start on 16
-// bytes, and caches that a tensor map describes.
+// Whether the tensor-core kernel takes a 16-bit call: caches that a tensor map describes, and more than 8
+// rows or wide heads.  Measured (us, this kernel / the
+// mma.sync one, 8 kv heads): 8 rows, 8 x 8192 keys, head_dim 64: 37.0 / 34.6; head_dim 128: 47.1 / 51.6;
+// 16 rows: 39.7 / 39.5 and 50.5 / 57.3; 32 rows: 42.0 / 50.7 and 53.1 / 69.6; 128 rows: 44.4 / 95.2 and
+// 59.4 / 133.2.
 static bool ta_takes_tc(const ns_tree_attn_t* p) {
   const int rows = p->T * (p->n_head / p->n_head_kv);
-  if (rows <= 32) return false;
-  if (!aligned_to(p->q, 16) || !aligned_to(p->out, 16) || !strides_multiple(p->q_stride, 3, 8) || !strides_multiple(p->o_stride, 3, 8))
-    return false;
+  if (rows <= 8 && p->head_dim <= 64) return false;
   const int64_t dims[3] = {p->B, p->n_head_kv, p->max_ctx};
   for (int i = 0; i < 3; ++i)
     for (const int64_t* s : {p->kc_stride, p->vc_stride})
@@ -716,6 +741,8 @@ static int ta_run_tc(const ns_tree_attn_t* p, void* ws, ns_stream_t stream, size
   t.a.tile_rows = MR;
   t.a.row_tiles = (rows + MR - 1) / MR;
   t.a.block = kTcAttnBlock;
+  t.a.vec = (aligned_to(p->q, 16) && strides_multiple(p->q_stride, 3, 8) ? 1 : 0) |
+            (aligned_to(p->out, 16) && strides_multiple(p->o_stride, 3, 8) ? 2 : 0);
   t.a.part_o = static_cast<float*>(ws);
   t.a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + o_bytes);
   int sms = 0;
