@@ -11,6 +11,8 @@
 // the heads of one token: one table slice, one division, for all of them.  The heads' elements are read
 // before the token's position is known (length, then depth in the tree, then the table's row: each
 // waits for the one before).  Rows that do not divide into octets on 16 bytes go pair by pair.
+#include <type_traits>
+
 #include "tree.cuh"
 
 namespace ns {
@@ -95,41 +97,50 @@ __device__ __forceinline__ RopeAt rope_at_token(const ns_rope_append_t& p, int64
 
 constexpr int kRopeRowThreads = 256;
 
-// NU: heads a thread reads side by side (gridDim.x > 1 shares a token's heads out when tokens are few)
-template <int DT, bool INTER, int NU>
+// NU: heads a thread reads side by side (gridDim.x > 1 shares a token's heads out when tokens are few).
+// CT: type of the caches.  The index arithmetic of a row is as long as its rotation, so the addresses of
+// the three kinds of rows run along and a row picks its own.
+template <int DT, int CT, bool INTER, int NU>
 __global__ void __launch_bounds__(kRopeRowThreads) rope_rows_kernel(const __grid_constant__ ns_rope_append_t p) {
+  constexpr int ES = DT == NS_F32 ? 4 : 2, CS = CT == NS_F32 ? 4 : 2;
   const int per = p.head_dim / 16, n_rot = p.rotary_dim / 16;  // units of a row, and the rotating ones
   const int row0 = threadIdx.x / per, u = threadIdx.x % per, step = kRopeRowThreads / per;
   const int nq = p.q ? p.n_head : 0, nk = p.k ? p.n_head_kv : 0, nv = p.v ? p.n_head_kv : 0, rows = nq + nk + nv;
   const bool rotates = u < n_rot;
   // first elements of the unit's octets
   const int d0 = !rotates || INTER ? 16 * u : 8 * u, d1 = !rotates || INTER ? 16 * u + 8 : p.rotary_dim / 2 + 8 * u;
+  const int first_row = row0 + blockIdx.x * step * NU, jump = step * NU * gridDim.x;
   griddep_wait();
   griddep_launch_dependents();
   for (int64_t tok = blockIdx.y; tok < (int64_t)p.B * p.T; tok += gridDim.y) {
     const int b = (int)(tok / p.T), t = (int)(tok % p.T);
-    const int64_t qo = b * p.q_stride[0] + t * p.q_stride[1], ko = b * p.k_stride[0] + t * p.k_stride[1],
-                  vo = b * p.v_stride[0] + t * p.v_stride[1];
+    // the row of each kind at index first_row of the list (q, k, v), and the way to the next
+    const char* qs = static_cast<const char*>(p.q) + (b * p.q_stride[0] + t * p.q_stride[1] + first_row * p.q_stride[2] + d0) * ES;
+    const char* ks = static_cast<const char*>(p.k) + (b * p.k_stride[0] + t * p.k_stride[1] + (first_row - nq) * p.k_stride[2] + d0) * ES;
+    const char* vs = static_cast<const char*>(p.v) + (b * p.v_stride[0] + t * p.v_stride[1] + (first_row - nq - nk) * p.v_stride[2] + d0) * ES;
+    const int64_t qstep = step * p.q_stride[2] * ES, kstep = step * p.k_stride[2] * ES, vstep = step * p.v_stride[2] * ES;
+    const int64_t ostep = step * p.qo_stride[2] * ES, kcstep = step * p.kc_stride[1] * CS, vcstep = step * p.vc_stride[1] * CS;
+    char *qd = nullptr, *kd = nullptr, *vd = nullptr;
     bool first = true;
     RopeAt at{0, 0, false};
     float c[8], s[8];
-    for (int r0 = row0 + blockIdx.x * step * NU; r0 - row0 < rows; r0 += step * NU * gridDim.x) {
+    for (int r0 = first_row; r0 - row0 < rows; r0 += jump) {
       uint4 raw[NU][DT == NS_F32 ? 4 : 2];
 #pragma unroll
       for (int k = 0; k < NU; ++k) {
         const int r = r0 + k * step;
+        const char* f = r < nq ? qs : r < nq + nk ? ks : vs;
+        qs += qstep, ks += kstep, vs += vstep;
         if (row0 >= step || r >= rows) continue;
-        const void* src = r < nq ? p.q : r < nq + nk ? p.k : p.v;
-        const int64_t so = r < nq ? qo + r * p.q_stride[2] : r < nq + nk ? ko + (r - nq) * p.k_stride[2] : vo + (r - nq - nk) * p.v_stride[2];
+        const char* f1 = f + (d1 - d0) * ES;
         if constexpr (DT == NS_F32) {
-          const float* f = static_cast<const float*>(src) + so;
-          raw[k][0] = *reinterpret_cast<const uint4*>(f + d0), raw[k][1] = *reinterpret_cast<const uint4*>(f + d0 + 4);
-          raw[k][2] = *reinterpret_cast<const uint4*>(f + d1), raw[k][3] = *reinterpret_cast<const uint4*>(f + d1 + 4);
+          raw[k][0] = *reinterpret_cast<const uint4*>(f), raw[k][1] = *reinterpret_cast<const uint4*>(f + 16);
+          raw[k][2] = *reinterpret_cast<const uint4*>(f1), raw[k][3] = *reinterpret_cast<const uint4*>(f1 + 16);
         } else {
-          const uint16_t* f = static_cast<const uint16_t*>(src) + so;
-          raw[k][0] = *reinterpret_cast<const uint4*>(f + d0), raw[k][1] = *reinterpret_cast<const uint4*>(f + d1);
+          raw[k][0] = *reinterpret_cast<const uint4*>(f), raw[k][1] = *reinterpret_cast<const uint4*>(f1);
         }
       }
+      if (gridDim.x > 1) qs += (jump / step - NU) * qstep, ks += (jump / step - NU) * kstep, vs += (jump / step - NU) * vstep;
       if (first) {
         first = false;
         at = rope_at_token(p, tok, b, t);
@@ -140,15 +151,19 @@ __global__ void __launch_bounds__(kRopeRowThreads) rope_rows_kernel(const __grid
           widen8<NS_F32>(cr, c);
           widen8<NS_F32>(sr, s);
         }
+        qd = static_cast<char*>(p.q_out) + (b * p.qo_stride[0] + t * p.qo_stride[1] + first_row * p.qo_stride[2] + d0) * ES;
+        kd = static_cast<char*>(p.k_cache) + (b * p.kc_stride[0] + (first_row - nq) * p.kc_stride[1] + at.slot * p.kc_stride[2] + d0) * CS;
+        vd = static_cast<char*>(p.v_cache) + (b * p.vc_stride[0] + (first_row - nq - nk) * p.vc_stride[1] + at.slot * p.vc_stride[2] + d0) * CS;
       }
 #pragma unroll
       for (int k = 0; k < NU; ++k) {
         const int r = r0 + k * step;
+        char* dst = r < nq ? qd : r < nq + nk ? kd : vd;
+        qd += ostep, kd += kcstep, vd += vcstep;
         if (row0 >= step || r >= rows || (r >= nq && !at.used)) continue;
         float x[8], y[8];
-        constexpr int H = DT == NS_F32 ? 2 : 1;
         widen8<DT>(raw[k], x);
-        widen8<DT>(raw[k] + H, y);
+        widen8<DT>(raw[k] + (DT == NS_F32 ? 2 : 1), y);
         if (rotates && r < nq + nk) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -160,22 +175,18 @@ __global__ void __launch_bounds__(kRopeRowThreads) rope_rows_kernel(const __grid
             d = e0 * c[j] + a0 * s[j];
           }
         }
-        void* dst;
-        int64_t dofs;
         if (r < nq) {
           if (!at.used)
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = y[j] = 0.f;
-          dst = p.q_out, dofs = b * p.qo_stride[0] + t * p.qo_stride[1] + r * p.qo_stride[2];
-        } else if (r < nq + nk) {
-          dst = p.k_cache, dofs = b * p.kc_stride[0] + (r - nq) * p.kc_stride[1] + at.slot * p.kc_stride[2];
+          store8(dst, DT, 0, x);
+          store8(dst, DT, d1 - d0, y);
         } else {
-          dst = p.v_cache, dofs = b * p.vc_stride[0] + (r - nq - nk) * p.vc_stride[1] + at.slot * p.vc_stride[2];
+          store8(dst, CT, 0, x);
+          store8(dst, CT, d1 - d0, y);
         }
-        const int dt = r < nq ? DT : p.cache_dtype;
-        store8(dst, dt, dofs + d0, x);
-        store8(dst, dt, dofs + d1, y);
       }
+      if (gridDim.x > 1) qd += (jump / step - NU) * ostep, kd += (jump / step - NU) * kcstep, vd += (jump / step - NU) * vcstep;
     }
   }
 }
@@ -252,15 +263,20 @@ static cudaError_t rope_launch(const ns_rope_append_t& p, bool vec, ns_stream_t 
   // Few tokens: a block for every part of a token's heads; more: a block a token, four heads in flight a
   // thread.  Measured for 80 heads of 128 in 16 bits (us, parts / whole): 32 tokens 2.5 / 3.2, 128 tokens
   // 4.4 / 3.2, 528 tokens 10.9 / 6.3.
-  if (tokens * parts <= 148) {
-    const dim3 grid((unsigned)parts, gy);
-    return p.interleaved ? launch_pdl(rope_rows_kernel<DT, true, 1>, grid, kRopeRowThreads, 0, stream, 1, p)
-                         : launch_pdl(rope_rows_kernel<DT, false, 1>, grid, kRopeRowThreads, 0, stream, 1, p);
+  const bool split = tokens * parts <= 148;
+  const dim3 grid(split ? (unsigned)parts : 1u, gy);
+  auto run = [&](auto ct, auto inter) {
+    constexpr int CT = decltype(ct)::value, NU = DT == NS_F32 ? 2 : 4;
+    constexpr bool INTER = decltype(inter)::value;
+    return split ? launch_pdl(rope_rows_kernel<DT, CT, INTER, 1>, grid, kRopeRowThreads, 0, stream, 1, p)
+                 : launch_pdl(rope_rows_kernel<DT, CT, INTER, NU>, grid, kRopeRowThreads, 0, stream, 1, p);
+  };
+  auto by_layout = [&](auto ct) { return p.interleaved ? run(ct, std::true_type{}) : run(ct, std::false_type{}); };
+  switch (p.cache_dtype) {
+    case NS_F32: return by_layout(std::integral_constant<int, NS_F32>{});
+    case NS_F16: return by_layout(std::integral_constant<int, NS_F16>{});
+    default: return by_layout(std::integral_constant<int, NS_BF16>{});
   }
-  constexpr int NU = DT == NS_F32 ? 2 : 4;
-  const dim3 grid(1, gy);
-  return p.interleaved ? launch_pdl(rope_rows_kernel<DT, true, NU>, grid, kRopeRowThreads, 0, stream, 1, p)
-                       : launch_pdl(rope_rows_kernel<DT, false, NU>, grid, kRopeRowThreads, 0, stream, 1, p);
 }
 
 }  // namespace ns
