@@ -5,7 +5,9 @@
 // (a 2- or 4-byte one where rows are not 16-byte aligned) of one head's rows and moves them in path
 // order.  The path ascends, so a row's target is never a later row's source (i < j gives
 // i <= path[i] < path[j]) and a thread may load a batch of rows ahead of its stores; columns are
-// independent, so nothing waits on another thread.
+// independent, so nothing waits on another thread.  Measured (device time of a call in a captured graph,
+// 36 layers of 8 heads): one sequence, 16 nodes, fp32, 3.0 us; 8 sequences, 64 nodes, bf16, 15 us
+// (50 MB, 3.4 TB/s): the loads of a batch of 8 rows wait for the path, then for memory.
 #include "tree.cuh"
 
 namespace ns {

@@ -13,6 +13,11 @@
 // a rejection costs a pass over the slice and an exchange of z, or, when no child is left, nothing of its
 // own: the pass that draws the token takes it out.  r at the other children follows by the same steps
 // on scalars.  (c needs no zero in the slice's q: w(c) = 0, since it was rejected with u < 1, and stays 0.)
+// Measured (device time of a call in a captured graph, vocabulary of 201,088): one chain of 8 nodes, fp32,
+// 12.8 us (two rows and the race: 2.4 MB); 16 trees of 32 nodes, bf16 logits and fp32 draft, 58 us, as long
+// as the longest walk among them.  A step of a walk is a pass of 4 to 7 thousand cycles (one load's latency,
+// then about ten instructions a logit) and an exchange of 2.5 to 3.5 thousand (reductions, cluster
+// barrier, remote reads): both are latency, the bytes would take a tenth.
 // The next token maximises r(x) / race(x): scores, unlike a cumulative sum over the vocabulary, do not
 // depend on the order of a summation.
 #include "tree.cuh"
