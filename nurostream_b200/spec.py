@@ -53,14 +53,27 @@ def _dense(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, dev) ->
 
 
 # Argument checks and the parameter block that follows from shapes, strides, types and devices are worked out once
-# per such layout and kept by it: a call looks its layout up, copies the block and fills in the pointers.
+# per such layout and kept by it: a call looks its layout up, copies the block and fills in the pointers.  Calls mostly
+# repeat the layout of the one before (layer after layer): it is compared first, which costs less than a hash.
 _LAYOUTS: dict = {}
+_LAST: dict = {}
 _MAX_LAYOUTS = 4096
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _sig(t: torch.Tensor | None):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _kept(key):
+    """The layout kept for this key (its first element names the operator), or None."""
+    last = _LAST.get(key[0])
+    if last is not None and last[0] == key:
+        return last[1]
+    layout = _LAYOUTS.get(key)
+    if layout is not None:
+        _LAST[key[0]] = (key, layout)
+    return layout
 
 
 def _keep(key, layout):
@@ -70,8 +83,8 @@ def _keep(key, layout):
     return layout
 
 
-def _stream(dev: torch.device) -> int:
-    return _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+def _stream(t: torch.Tensor) -> int:
+    return _raw_stream(t.get_device()) if _raw_stream is not None else torch.cuda.current_stream(t.device).cuda_stream
 
 
 def _ptr(t: torch.Tensor | None):
@@ -155,7 +168,7 @@ def _rope_layout(q, k, v, q_out, kc, vc, cos, sin, lens, parents, positions, rot
 def _rope_call(q, k, v, q_out, kc, vc, cos, sin, lens, parents, positions, rotary_dim, interleaved) -> None:
     key = ("rope", _sig(q), _sig(k), _sig(v), _sig(q_out), _sig(kc), _sig(vc), _sig(cos), _sig(sin), _sig(lens),
            _sig(parents), _sig(positions), rotary_dim, interleaved)
-    image = _LAYOUTS.get(key)
+    image = _kept(key)
     if image is None:
         image = _keep(key, _rope_layout(q, k, v, q_out, kc, vc, cos, sin, lens, parents, positions, rotary_dim, interleaved))
     p = _lib.RopeAppendParams.from_buffer_copy(image)
@@ -164,7 +177,7 @@ def _rope_call(q, k, v, q_out, kc, vc, cos, sin, lens, parents, positions, rotar
     p.q, p.q_out = q.data_ptr(), q_out.data_ptr()
     if kc is not None:
         p.k, p.v, p.k_cache, p.v_cache = k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr()
-    _lib.call("ns_rope_append", C.byref(p), _stream(q.device))
+    _lib.call("ns_rope_append", C.byref(p), _stream(q))
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -237,7 +250,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     """
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
     key = ("attn", _sig(q), _sig(k_cache), _sig(v_cache), _sig(o), _sig(lens), _sig(parents), _sig(sinks), window, scale)
-    layout = _LAYOUTS.get(key)
+    layout = _kept(key)
     if layout is None:
         layout = _keep(key, _attn_layout(q, k_cache, v_cache, o, lens, parents, sinks, window, scale))
     image, ws_bytes = layout
@@ -245,7 +258,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     p.lens, p.parents, p.sinks = lens.data_ptr(), _ptr(parents), _ptr(sinks)
     p.q, p.k_cache, p.v_cache, p.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr()
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-    _lib.call("ns_tree_attn", C.byref(p), ws.data_ptr(), ws_bytes, _stream(q.device))
+    _lib.call("ns_tree_attn", C.byref(p), ws.data_ptr(), ws_bytes, _stream(q))
     return o
 
 
@@ -286,7 +299,7 @@ def verify_tree(tokens: torch.Tensor, logits: torch.Tensor, uniforms: torch.Tens
     """
     key = ("verify", _sig(tokens), _sig(logits), _sig(uniforms), _sig(race), _sig(parents), _sig(draft_probs),
            _sig(temperature))
-    image = _LAYOUTS.get(key)
+    image = _kept(key)
     if image is None:
         image = _keep(key, _verify_layout(tokens, logits, uniforms, race, parents, draft_probs, temperature))
     B, T = tokens.shape
@@ -297,7 +310,7 @@ def verify_tree(tokens: torch.Tensor, logits: torch.Tensor, uniforms: torch.Tens
     p.tokens, p.logits, p.uniforms, p.race = tokens.data_ptr(), logits.data_ptr(), uniforms.data_ptr(), race.data_ptr()
     p.parents, p.draft_probs, p.temperature = _ptr(parents), _ptr(draft_probs), _ptr(temperature)
     p.path, p.n_accepted, p.next_token = path.data_ptr(), n_acc.data_ptr(), nxt.data_ptr()
-    _lib.call("ns_tree_verify", C.byref(p), _stream(logits.device))
+    _lib.call("ns_tree_verify", C.byref(p), _stream(logits))
     return path, n_acc, nxt
 
 
@@ -337,7 +350,7 @@ def commit_path(caches, lens: torch.Tensor, path: torch.Tensor, n_accepted: torc
     k0, v0, n = ks[0], vs[0], len(ks)
     out = torch.empty_like(lens) if new_lens is None else new_lens
     key = ("commit", n, _sig(k0), _sig(v0), _sig(lens), _sig(path), _sig(n_accepted), _sig(out))
-    image = _LAYOUTS.get(key)
+    image = _kept(key)
     if image is None:
         image = _keep(key, _commit_layout(n, k0, v0, lens, path, n_accepted, out))
     stride = torch.Tensor.stride
@@ -348,5 +361,5 @@ def commit_path(caches, lens: torch.Tensor, path: torch.Tensor, n_accepted: torc
     p.lens, p.path, p.n_accepted, p.new_lens = lens.data_ptr(), path.data_ptr(), n_accepted.data_ptr(), out.data_ptr()
     ptr = torch.Tensor.data_ptr
     p.k_cache[:n], p.v_cache[:n] = list(map(ptr, ks)), list(map(ptr, vs))
-    _lib.call("ns_path_commit", C.byref(p), _stream(k0.device))
+    _lib.call("ns_path_commit", C.byref(p), _stream(k0))
     return out
