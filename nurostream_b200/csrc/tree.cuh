@@ -60,7 +60,6 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, int threads, 
 }
 
 inline bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
-__device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 inline bool strides_multiple(const int64_t* s, int n, int64_t of) {
   for (int i = 0; i < n; ++i)
     if (s[i] % of) return false;

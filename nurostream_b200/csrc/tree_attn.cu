@@ -60,7 +60,7 @@ struct TaArgs {
 struct TaShared {
   uint64_t anc[kTreeMax];   // of the sequence at hand
   int depth[kTreeMax], par[kTreeMax];
-  int max_depth, bad_lo, bad_hi;
+  int max_depth;
   uint32_t bad_keys[4];     // keys of the block whose values are not finite and not seen by all
   float wm[kTaWarps][16], wl[kTaWarps][16];
 };

@@ -530,3 +530,37 @@ def test_refusals():
         spec.commit_path([(kc, kc), (kc, kc.float())], lens, tok, lens)
     with pytest.raises(_lib.NsError):
         spec.commit_path([(kc, kc)], lens, tok, lens, new_lens=lens)
+
+
+# ------------------------------------------------------------------------------------------ the tensor-core kernel
+
+
+@pytest.mark.parametrize("B,T,hq,hkv,hd,window", [(130, 8, 8, 2, 64, 0), (60, 20, 16, 1, 64, 9), (40, 33, 8, 1, 128, 0),
+                                                  (150, 5, 8, 2, 128, 4)])
+def test_many_items_in_a_run(B, T, hq, hkv, hd, window):
+    """Runs of many short items: several whole items in a row, one and two slots of rows, more than one tile."""
+    q, kc, vc, lens, par, sk = _attn_case(B, T, hq, hkv, hd, 30, True, True, BF16)
+    want, smax, vmax = oracle.attention(f64(q), f64(kc), f64(vc), lens.cpu(), par.cpu(), f64(sk), window, hd ** -0.5)
+    out = spec.tree_attention(q, kc, vc, lens, par, sinks=sk, window=window)
+    assert (np.abs(f64(out) - want) <= _attn_tol(BF16, smax, vmax, want)).all()
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("hq,hkv,hd", [(4, 2, 64), (32, 4, 64), (64, 4, 128)])
+def test_bad_branches_of_big_trees(dt, hq, hkv, hd):
+    """Nodes whose values are not finite, in trees of one and several tiles of rows over a cut context."""
+    T, n = 64, 700
+    q, kc, vc, lens, par, _ = _attn_case(2, T, hq, hkv, hd, n, True, False, dt)
+    want = spec.tree_attention(q, kc, vc, lens, par)
+    bad = {0: (9, 40), 1: (5,)}
+    trees = [oracle.tree(p, T) for p in par.cpu()]
+    for b, nodes in bad.items():
+        for t in nodes:
+            vc[b, :, int(lens[b]) + t] = float("nan")
+    out = spec.tree_attention(q, kc, vc, lens, par)
+    for b, nodes in bad.items():
+        for t, anc in enumerate(trees[b]):
+            if anc is not None and set(nodes) & set(anc):
+                assert torch.isnan(out[b, t]).all()
+            else:
+                assert torch.equal(out[b, t], want[b, t])
