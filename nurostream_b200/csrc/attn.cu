@@ -38,8 +38,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 // Barrier over every thread of every CTA of the cluster, ordering shared-memory writes before it
-// against reads after it (a launch without clusters is a cluster of one CTA).
+// against reads after it (a launch without clusters is a cluster of one CTA).  The instructions are
+// .aligned: the warp's threads come to them together.
 __device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Address of the same shared-memory variable in the CTA of cluster rank r.

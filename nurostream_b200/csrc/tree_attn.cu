@@ -521,6 +521,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
               if (pv[0] != 0.f) o[n][j] = fmaf(pv[0], v, o[n][j]);
               if (pv[1] != 0.f) o[n][2 + j] = fmaf(pv[1], v, o[n][2 + j]);
             }
+          __syncwarp();  // the products of the next keys are .aligned
         }
       }
     }

@@ -362,6 +362,9 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
           if (dep - S.depth[nd] >= p.window) vis &= ~(1ull << nd);
         }
       }
+      // The tensor-memory instructions below are .aligned: the whole warp has to be at them together, and the
+      // code above (rows copied and not, loops as long as a row's ancestors) lets lanes part.
+      __syncwarp();
       {
         uint32_t z[32];
 #pragma unroll
@@ -477,6 +480,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
                   if (pv != 0.f && 32 * c + i < p.head_dim) o[i] = fmaf(pv, load_float(p.v_cache, DT, vrow + 32 * c + i), o[i]);
+                __syncwarp();  // lanes whose row does not see the key skipped the loads
                 tmem_st_x32(o_col(s) + lane_base + 32 * c, reinterpret_cast<const uint32_t*>(o));
               }
               tmem_wait_st();
@@ -522,6 +526,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
       constexpr int NC = HD / 32;
 #pragma unroll 1
       for (int c = PAIR ? 0 : s * (NC / 2); c < (PAIR ? NC : (s + 1) * (NC / 2)); ++c) {
+        __syncwarp();  // lanes without a row do not store (here and above)
         float o[32];
         tmem_ld_x32(o_col(PAIR ? s : 0) + lane_base + 32 * c, o);
         if constexpr (!PAIR) {
@@ -534,8 +539,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
         } else {
           tmem_wait_ld_x32(o);
         }
-        if (!has_row) continue;
-        if (whole) {
+        if (has_row && whole) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8)
             if (32 * c + i < p.head_dim) {
@@ -549,12 +553,13 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
                 for (int k = 0; k < 8; ++k) store_float(p.out, DT, oo + 32 * c + i + k, y[k]);
               }
             }
-        } else {
+        } else if (has_row) {
           float4* po = reinterpret_cast<float4*>(a.part_o + pr * HD + 32 * c);
 #pragma unroll
           for (int i = 0; i < 8; ++i) po[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
+      __syncwarp();
       tc_fence_before();
       return true;
     });

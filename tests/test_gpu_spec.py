@@ -564,3 +564,33 @@ def test_bad_branches_of_big_trees(dt, hq, hkv, hd):
                 assert torch.isnan(out[b, t]).all()
             else:
                 assert torch.equal(out[b, t], want[b, t])
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("B,T,hq,hkv,hd,n,window,bad", [
+    (1, 5, 3, 1, 128, 700, 9, False),      # 15 rows: one warp's half, cut between runs
+    (2, 9, 10, 2, 128, 300, 4, True),      # 45 rows: a warp and a part of one
+    (3, 27, 6, 2, 64, 90, 0, True),        # 81 rows
+    (40, 11, 6, 1, 64, 20, 3, True),       # 66 rows, whole items
+    (1, 37, 7, 1, 128, 900, 11, True),     # 259 rows: three of a second tile
+    (2, 61, 5, 1, 120, 140, 6, False),     # 305 rows
+])
+def test_rows_that_end_inside_a_warp(B, T, hq, hkv, hd, n, window, bad, dt):
+    """Lanes of one warp with and without a row, with trees of different depth under a window, and values that only
+    some of them see."""
+    q, kc, vc, lens, par, sk = _attn_case(B, T, hq, hkv, hd, n, True, True, dt)
+    trees = [oracle.tree(p, T) for p in par.cpu()]
+    node = T // 2
+    if bad:
+        for b in range(B):
+            vc[b, :, int(lens[b]) + node] = 0
+    want, smax, vmax = oracle.attention(f64(q), f64(kc), f64(vc), lens.cpu(), par.cpu(), f64(sk), window, hd ** -0.5)
+    if bad:  # NaN where the plain values have zeros: rows that see it become NaN, the others stay
+        for b in range(B):
+            vc[b, :, int(lens[b]) + node] = float("nan")
+    out = f64(spec.tree_attention(q, kc, vc, lens, par, sinks=sk, window=window))
+    ok = np.abs(out - want) <= _attn_tol(dt, smax, vmax, want)
+    for b in range(B):
+        for t, anc in enumerate(trees[b]):
+            sees = bad and anc is not None and node in anc and (not window or len(anc) - 1 - anc.index(node) < window)
+            assert np.isnan(out[b, t]).all() if sees else ok[b, t].all(), (b, t)
