@@ -394,7 +394,7 @@ int ns_embed(const void* table, int dtype, int64_t rows, int H, const int32_t* t
  * Generalises neurostream/compute/ops.py:136-151 `apply_rope` and
  * neurostream/model/qwen3.py:74-85 `KVCache.append` to batches, trees, partial
  * and interleaved rotation and 16-bit caches.
- * Tables: fp32, n_pos rows of at least rotary_dim/2 columns, row stride
+ * Tables: fp32, n_pos (at least 1) rows of at least rotary_dim/2 columns, row stride
  * table_stride.  positions (B x T int32) replaces lens + depth as the table row
  * when given.  q, k or v may be NULL (nothing is done for it); q_out may be q.
  * Rows of unused nodes: q_out is zero, the cache is left alone.  Any T when

@@ -300,6 +300,8 @@ extern "C" int ns_rope_append(const ns_rope_append_t* p, ns_stream_t stream) {
     return fail(NS_ERR_UNSUPPORTED, "ns_rope_append: a tree of %d nodes (at most %d)", p->T, NS_TREE_MAX_NODES);
   if (p->B == 0 || p->T == 0) return NS_OK;
   if (!p->lens || !p->rope_cos || !p->rope_sin) return fail(NS_ERR_INVALID, "ns_rope_append: null lens or tables");
+  // (a node whose position is no row of the tables reads row 0 and drops it)
+  if (p->n_pos == 0) return fail(NS_ERR_INVALID, "ns_rope_append: tables without rows");
   if ((p->q && !p->q_out) || (p->k && !p->k_cache) || (p->v && !p->v_cache))
     return fail(NS_ERR_INVALID, "ns_rope_append: an input without its output");
   if ((int64_t)(p->n_head + 2 * (int64_t)p->n_head_kv) * p->head_dim > (1 << 28))

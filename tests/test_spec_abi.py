@@ -140,3 +140,10 @@ def test_commit_refusals(lib, kw, status):
 def test_nothing_to_verify_or_commit(lib):
     assert lib.ns_tree_verify(C.byref(_verify(B=0)), None) == 0
     assert lib.ns_path_commit(C.byref(_commit(B=0)), None) == 0
+
+
+def test_rope_refuses_tables_without_rows(lib):
+    """A node without a position reads row 0 of the tables: there has to be one."""
+    assert lib.ns_rope_append(C.byref(_rope(n_pos=0)), None) == -1
+    assert b"tables without rows" in lib.ns_last_error()
+    assert lib.ns_rope_append(C.byref(_rope(n_pos=0, T=0)), None) == 0
