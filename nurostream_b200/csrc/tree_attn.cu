@@ -61,7 +61,7 @@ struct TaShared {
   uint64_t anc[kTreeMax];   // of the sequence at hand
   int depth[kTreeMax], par[kTreeMax];
   int max_depth;
-  uint32_t bad_keys[4];     // keys of the block whose values are not finite and not seen by all
+  uint32_t bad_keys[2][4];  // keys of the block whose values the products cannot take; of every other block
   float wm[kTaWarps][16], wl[kTaWarps][16];
 };
 
@@ -162,11 +162,15 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo, both rounded to the 11 significant bits of tf32 (the tensor core drops the bits below)
+// x = hi + lo: hi is x rounded to the 11 significant bits of tf32, lo what is left of it, of which the tensor core
+// drops the bits below its own 11 (at most the last bit of x, 2^-23 of it, which rounding would be off by too).
+// NaN stays NaN in one part or both.  Infinities and values that round to one (kTf32Top and above) come out
+// as parts whose products add to NaN: they are looked for and done in plain fp32.
 __device__ __forceinline__ void tf32_split(uint32_t x, uint32_t& hi, uint32_t& lo) {
   hi = (x + 0x1000u) & 0xFFFFE000u;
-  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi)) + 0x1000u;
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
 }
+constexpr uint32_t kTf32Top = 0x7F7FF000u;
 template <int DT>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
   if constexpr (DT == NS_F16) {
@@ -183,14 +187,15 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Whether 16 bytes of shared memory hold a value that is not finite (an exponent of ones: adding one to
-// it carries into the sign's place, which the mask has cleared).
+// Whether 16 bytes of shared memory hold a value that the products cannot take: one that is not finite (in 16 bits:
+// an exponent of ones, to which adding one carries into the sign's place, that the mask has cleared), in fp32
+// also one that tf32_split makes infinite (kTf32Top carries there with what is added).
 template <int DT>
 __device__ __forceinline__ uint32_t not_finite(uint32_t saddr) {
   uint32_t w[4];
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(saddr) : "memory");
-  constexpr uint32_t m = DT == NS_F32 ? 0x7F800000u : DT == NS_F16 ? 0x7C007C00u : 0x7F807F80u;
-  constexpr uint32_t one = DT == NS_F32 ? 0x00800000u : DT == NS_F16 ? 0x04000400u : 0x00800080u;
+  constexpr uint32_t m = DT == NS_F32 ? 0x7FFFFFFFu : DT == NS_F16 ? 0x7C007C00u : 0x7F807F80u;
+  constexpr uint32_t one = DT == NS_F32 ? 0x80000000u - kTf32Top : DT == NS_F16 ? 0x04000400u : 0x00800080u;
   constexpr uint32_t top = DT == NS_F32 ? 0x80000000u : 0x80008000u;
   return (((w[0] & m) + one) | ((w[1] & m) + one) | ((w[2] & m) + one) | ((w[3] & m) + one)) & top;
 }
@@ -240,6 +245,9 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
       cp_async16_z(dv + off, vb + key * p.vc_stride[2] * EL + cc * 16, ok);
     }
   };
+
+  if (tid < 8) S.bad_keys[tid >> 2][tid & 3] = 0;
+  int scan = 0;  // which of bad_keys the block uses
 
   int64_t ul = u0;
 #pragma unroll
@@ -341,23 +349,24 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
     const int k0 = sp.lo + at.blk * BN;
     // a block needs no mask when every row sees all of it
     const bool masked = k0 + BN > sp.len || (p.window > 0 && sp.len + S.max_depth - k0 >= p.window);
-    if (masked) {
-      // values that not every row sees may hold anything: rows of the block that are not finite are
-      // set to zero here and added, for the rows that see them, from the cache below
-      if (tid < 4) S.bad_keys[tid] = 0;
-      __syncthreads();
+    // Values that not every row sees may hold anything, and fp32 products take no infinities: rows of the block that
+    // hold such values are set to zero here and added, for the rows that see them, from the cache below.
+    const bool look = DT == NS_F32 || masked;
+    if (look) {
+      scan ^= 1;
+      if (tid < 4) S.bad_keys[scan ^ 1][tid] = 0;  // for the next block that looks; its last readers are past the barrier
 #pragma unroll 4
       for (int i = 0; i < BN * CH / kTaThreads; ++i) {
         const int c = tid + i * kTaThreads;
-        if (not_finite<DT>(vs + c * 16)) atomicOr(&S.bad_keys[c / CH >> 5], 1u << (c / CH & 31));
+        if (not_finite<DT>(vs + c * 16)) atomicOr(&S.bad_keys[scan][c / CH >> 5], 1u << (c / CH & 31));
       }
       __syncthreads();
       uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < BN / 32; ++i) any |= S.bad_keys[i];
+      for (int i = 0; i < BN / 32; ++i) any |= S.bad_keys[scan][i];
       if (any) {
         for (int c = tid; c < BN * CH; c += kTaThreads)
-          if (S.bad_keys[c / CH >> 5] >> (c / CH & 31) & 1) sts128(vs + c * 16, 0, 0, 0, 0);
+          if (S.bad_keys[scan][c / CH >> 5] >> (c / CH & 31) & 1) sts128(vs + c * 16, 0, 0, 0, 0);
         __syncthreads();
       }
     }
@@ -420,6 +429,32 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
             }
             if (!see) s[n][j] = -INFINITY;
           }
+      }
+      if constexpr (DT == NS_F32) {  // scores that came out as NaN: the products may not have taken q or k
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < SB / 8; ++n) sum[0] += s[n][0] + s[n][1], sum[1] += s[n][2] + s[n][3];
+        if (__any_sync(0xffffffffu, (anc[0] && sum[0] != sum[0]) || (anc[1] && sum[1] != sum[1]))) {
+#pragma unroll 1
+          for (int e = 0; e < SB / 2; ++e) {
+            const int n = e >> 2, j = e & 3, r = at.rt * MR + wm * 16 + g + 8 * (j >> 1);
+            float x = 0.f;
+#pragma unroll
+            for (int i = 0; i < SB / 2; ++i) x = i == e ? s[i >> 2][i & 3] : x;
+            if (x != x && (j >> 1 ? anc[1] : anc[0])) {
+              const float* q = static_cast<const float*>(p.q) + at.b * p.q_stride[0] + r / a.rep * p.q_stride[1] +
+                               (at.h * a.rep + r % a.rep) * p.q_stride[2];
+              const float* k = static_cast<const float*>(p.k_cache) + at.b * p.kc_stride[0] + at.h * p.kc_stride[1] +
+                               (int64_t)(k0 + kr + n * 8 + 2 * tq + (j & 1)) * p.kc_stride[2];
+              x = 0.f;
+#pragma unroll 8
+              for (int d = 0; d < p.head_dim; ++d) x = fmaf(q[d], k[d], x);
+            }
+#pragma unroll
+            for (int i = 0; i < SB / 2; ++i)
+              if (i == e) s[i >> 2][i & 3] = x;
+          }
+        }
       }
 #pragma unroll
       for (int n = 0; n < SB / 8; ++n) {
@@ -497,8 +532,8 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
           }
         }
       }
-      if (masked) {  // values that are not finite, for the rows that see them
-        uint32_t bad = S.bad_keys[kr >> 5] >> (kr & 31);
+      if (look) {  // the values left out, for the rows that see them
+        uint32_t bad = S.bad_keys[scan][kr >> 5] >> (kr & 31);
         if constexpr (SB < 32) bad &= (1u << SB) - 1;
         while (bad) {
           const int kk = __ffs(bad) - 1;

@@ -594,3 +594,63 @@ def test_rows_that_end_inside_a_warp(B, T, hq, hkv, hd, n, window, bad, dt):
         for t, anc in enumerate(trees[b]):
             sees = bad and anc is not None and node in anc and (not window or len(anc) - 1 - anc.index(node) < window)
             assert np.isnan(out[b, t]).all() if sees else ok[b, t].all(), (b, t)
+
+
+# ------------------------------------------------------------------------------------------ values that are not finite
+
+def _put(t, value):
+    """value into every element of an fp32 view; "nan" as the GPU writes it (Python would make another one)."""
+    if value == "nan":
+        bits = torch.full(t.shape, 0x7FFFFFFF, **I32)
+        t.copy_(bits.view(F32))
+        assert (t.clone().view(torch.int32) == 0x7FFFFFFF).all()
+    else:
+        t.fill_(value)
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("T,hq", [(1, 2), (11, 12), (40, 8)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_ignores_the_types_extremes(T, hq, dt, sign):
+    """Masked slots that hold the largest or lowest value of the type."""
+    hole = sign * torch.finfo(dt).max
+    args = (3, T, hq, 2, 64, 150, True, True)
+    q, kc, vc, lens, par, sk = _attn_case(*args, dt)
+    want = spec.tree_attention(q, kc, vc, lens, par, sinks=sk, window=60)
+    q, kc, vc, lens, par, sk = _attn_case(*args, dt, hole=hole)
+    kc[0, :, :30], vc[0, :, :30] = hole, hole
+    assert torch.equal(want, spec.tree_attention(q, kc, vc, lens, par, sinks=sk, window=60))
+
+
+F32_ROWS = [(1, 2, 2, 64), (2, 8, 2, 64), (4, 12, 2, 128), (9, 12, 2, 64), (20, 12, 2, 128)]  # T, hq, hkv, hd: 1 to 120 rows
+
+
+@pytest.mark.parametrize("T,hq,hkv,hd", F32_ROWS)
+@pytest.mark.parametrize("key", [10, 198])      # in a block that every row sees, and in one with a mask
+def test_fp32_attention_with_a_seen_nan_or_infinity(T, hq, hkv, hd, key):
+    q, kc, vc, lens, _, _ = _attn_case(1, T, hq, hkv, hd, 200, False, False, F32)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    rep, base = hq // hkv, spec.tree_attention(q, kc, vc, lens)
+    want, smax, vmax = oracle.attention(f64(q), f64(kc), f64(vc), lens.cpu(), None, None, 0, hd ** -0.5)
+    k0, v0 = kc.clone(), vc.clone()
+
+    _put(kc[0, 0, key, 3], "nan")               # every row of the first kv head, none of the others
+    out = spec.tree_attention(q, kc, vc, lens)
+    assert torch.isnan(out[:, :, :rep]).all() and torch.equal(out[:, :, rep:], base[:, :, rep:])
+    kc.copy_(k0)
+
+    for value in ("nan", float("inf"), float("-inf")):   # one column of them
+        _put(vc[0, 0, key, 5], value)
+        out = spec.tree_attention(q, kc, vc, lens)
+        hit = out[:, :, :rep, 5]
+        assert torch.isnan(hit).all() if value == "nan" else (hit == value).all()
+        out[:, :, :rep, 5] = base[:, :, :rep, 5]
+        assert torch.equal(out[:, :, rep:], base[:, :, rep:])
+        assert (np.abs(f64(out) - want) <= _attn_tol(F32, smax, vmax, want)).all()
+        vc.copy_(v0)
+
+    kc[0, 0, key, 0] = float("-inf")            # against positive queries: a probability of zero
+    out = spec.tree_attention(q, kc, vc, lens)
+    gone, _, _ = oracle.attention(f64(q), f64(kc), f64(vc), lens.cpu(), None, None, 0, hd ** -0.5)
+    assert np.isfinite(gone).all() and (np.abs(f64(out) - gone) <= _attn_tol(F32, smax, vmax, gone)).all()
+    kc.copy_(k0)
