@@ -65,6 +65,28 @@ struct TaShared {
   float wm[kTaWarps][16], wl[kTaWarps][16];
 };
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Probabilities are relative to the running maximum and are divided by their sum last, so a running output is up to
+// as many times a value as there are keys: the largest values would overflow where the result does not.  In the
+// types that have fp32's range all of them are 2^-kShift of that, which is exact (2^24 keys, each up to 2^8:
+// the tensor-core kernel's maximum may lag), and a sink's share is scaled alike.  fp16's values cannot get there.
+template <int DT>
+constexpr float kTaShift = DT == NS_F16 ? 0.f : 32.f;
+static_assert(kTaShift<NS_F32> == 32.f, "0x1p-32f in tree_attn_kernel");
+
+// The factor of a row: one over its sum l relative to maximum m, with the head's sink (in units of log2) in it.
+template <int DT>
+__device__ __forceinline__ float ta_row_scale(float m, float l, const float* sinks, int h) {
+  if (!sinks) return 1.f / l;
+  const float sk = sinks[h] * 1.4426950408889634f, mm = fmaxf(m, sk);
+  return ex2(m - mm) / fmaf(l, ex2(m - mm), ex2(sk - mm - kTaShift<DT>));
+}
+
 // Keys [lo, hi) of sequence b that any node may see, and how many blocks they are.
 struct TaSpan {
   int lo, hi, len;
@@ -180,11 +202,6 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Whether 16 bytes of shared memory hold a value that the products cannot take: one that is not finite (in 16 bits:
@@ -479,9 +496,11 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float x = s[n][j];
-          const float e = DT == NS_F32 && x != -INFINITY ? fmaf(x, sc_lo, fmaf(x, sc_hi, -ref[j >> 1]))
-                                                         : fmaf(x, sc_hi, -ref[j >> 1]);
-          s[n][j] = ex2(e);
+          // (kTaShift in fp32 as a factor: added to the exponent it would cost that its last bits)
+          const float e = DT != NS_F32      ? fmaf(x, sc_hi, -kTaShift<DT> - ref[j >> 1])
+                          : x != -INFINITY ? fmaf(x, sc_lo, fmaf(x, sc_hi, -ref[j >> 1]))
+                                           : -INFINITY;
+          s[n][j] = DT == NS_F32 ? ex2(e) * 0x1p-32f : ex2(e);
           l[j >> 1] += s[n][j];
         }
       if constexpr (DT != NS_F32) {
@@ -608,15 +627,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
           const int row = at.rt * MR + r, t = row / a.rep, h = at.h * a.rep + row % a.rep;
           if (whole) {
             const bool live = S.anc[t] != 0 && mt != -INFINITY;
-            float scale = 0.f;
-            if (live) {
-              if (p.sinks) {
-                const float sk = p.sinks[h] * 1.4426950408889634f, mm = fmaxf(mt, sk);
-                scale = ex2(mt - mm) / fmaf(lt, ex2(mt - mm), ex2(sk - mm));
-              } else {
-                scale = 1.f / lt;
-              }
-            }
+            const float scale = live ? ta_row_scale<DT>(mt, lt, p.sinks, h) : 0.f;
             const int64_t oo = at.b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i)
@@ -640,15 +651,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
           const int row = at.rt * MR + r, t = row / a.rep, h = at.h * a.rep + row % a.rep;
           if (whole) {
             const bool live = anc[i] != 0 && m[i] != -INFINITY;
-            float scale = 0.f;
-            if (live) {
-              if (p.sinks) {
-                const float sk = p.sinks[h] * 1.4426950408889634f, mm = fmaxf(m[i], sk);
-                scale = ex2(m[i] - mm) / fmaf(l[i], ex2(m[i] - mm), ex2(sk - mm));
-              } else {
-                scale = 1.f / l[i];
-              }
-            }
+            const float scale = live ? ta_row_scale<DT>(m[i], l[i], p.sinks, h) : 0.f;
             const int64_t oo = at.b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
 #pragma unroll
             for (int n = 0; n < HD / 8; ++n)
@@ -723,11 +726,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const _
   auto finish = [&](int r, float mt, float lt, float (&acc)[V]) {  // one row out
     const int row = rt * MR + r, t = row / a.rep, h = hk * a.rep + row % a.rep;
     const bool live = mt != -INFINITY;  // an unused node's parts say -inf
-    float scale = live ? 1.f / lt : 0.f;
-    if (live && p.sinks) {
-      const float sk = p.sinks[h] * 1.4426950408889634f, mm = fmaxf(mt, sk);
-      scale = ex2(mt - mm) / fmaf(lt, ex2(mt - mm), ex2(sk - mm));
-    }
+    const float scale = live ? ta_row_scale<DT>(mt, lt, p.sinks, h) : 0.f;
     const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2] + lane * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = live ? acc[j] * scale : 0.f;

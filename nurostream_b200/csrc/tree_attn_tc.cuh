@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
           l *= f;
         }
         if (move) m = top;
-        const float ref = m == -INFINITY ? 0.f : m;
+        const float ref = (m == -INFINITY ? 0.f : m) + kTaShift<DT>;
         uint64_t sum[2] = {0, 0};
         const uint64_t sc2 = pair2(sc, sc), ref2 = pair2(-ref, -ref);
         // probabilities, rounded to 16 bits: half an ulp each, as large as the output's own rounding
@@ -511,14 +511,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
         l = ml[128 + row] * f0 + ml[384 + row] * f1;
       }
       const bool whole = it.n == it.pos.nblk, live = used && m != -INFINITY;
-      float scale = 1.f;
-      if (whole) {
-        scale = live ? 1.f / l : 0.f;
-        if (live && p.sinks) {
-          const float sink = p.sinks[h] * 1.4426950408889634f, mm = fmaxf(m, sink);
-          scale = ex2(m - mm) / fmaf(l, ex2(m - mm), ex2(sink - mm));
-        }
-      }
+      const float scale = whole && live ? ta_row_scale<DT>(m, l, p.sinks, h) : 0.f;
       const int slot = 2 * blockIdx.x + (u - it.pos.blk <= u0 ? 0 : 1);
       const int64_t pr = (int64_t)slot * MR + (PAIR ? s * 128 : 0) + row;
       const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];

@@ -654,3 +654,42 @@ def test_fp32_attention_with_a_seen_nan_or_infinity(T, hq, hkv, hd, key):
     gone, _, _ = oracle.attention(f64(q), f64(kc), f64(vc), lens.cpu(), None, None, 0, hd ** -0.5)
     assert np.isfinite(gone).all() and (np.abs(f64(out) - gone) <= _attn_tol(F32, smax, vmax, gone)).all()
     kc.copy_(k0)
+
+
+@pytest.mark.parametrize("T,hq,hkv,hd", F32_ROWS)
+@pytest.mark.parametrize("key", [10, 198])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_fp32_attention_takes_the_largest_values(T, hq, hkv, hd, key, sign):
+    top = sign * torch.finfo(F32).max
+    q, kc, vc, lens, _, _ = _attn_case(1, T, hq, hkv, hd, 200, False, False, F32)
+    kc[0, 0, key, 0], q[..., 0] = top, 2.0 ** -126      # their product is modest
+    want, smax, vmax = oracle.attention(f64(q), f64(kc), f64(vc), lens.cpu(), None, None, 0, hd ** -0.5)
+    out = spec.tree_attention(q, kc, vc, lens)
+    assert (np.abs(f64(out) - want) <= _attn_tol(F32, smax, vmax, want)).all()
+    vc[0, 0, key, 5] = top
+    q[..., 0], kc[..., 0] = top, 2.0 ** -126            # and the other way round
+    want, smax, _ = oracle.attention(f64(q), f64(kc), f64(vc), lens.cpu(), None, None, 0, hd ** -0.5)
+    out = f64(spec.tree_attention(q, kc, vc, lens))
+    hit = (0, slice(None), slice(0, hq // hkv), 5)
+    assert (np.abs(out - want)[hit] <= _attn_tol(F32, smax, abs(top), want[hit])).all()
+    out[hit] = want[hit]
+    assert (np.abs(out - want) <= _attn_tol(F32, smax, vmax, want)).all()
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("T,hq,hkv,hd", [(1, 2, 2, 64), (4, 12, 2, 128), (20, 12, 2, 64), (33, 16, 2, 64)])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_attention_sums_of_large_values(T, hq, hkv, hd, sinks, dt):
+    """One column of values that would overflow if they were added up before the division by the probabilities' sum."""
+    big = torch.finfo(dt).max / 2
+    q, kc, vc, lens, _, sk = _attn_case(2, T, hq, hkv, hd, 300, False, sinks, dt)
+    vc[..., 5] = big
+    want, smax, vmax = oracle.attention(f64(q), f64(kc), f64(vc), lens.cpu(), None, None if sk is None else f64(sk), 0,
+                                        hd ** -0.5)
+    out = f64(spec.tree_attention(q, kc, vc, lens, sinks=sk))
+    assert (np.abs(out - want)[..., 5] <= _attn_tol(dt, smax, big, want[..., 5])).all()
+    vc[..., 5] = 1.0
+    want, smax, vmax = oracle.attention(f64(q), f64(kc), f64(vc), lens.cpu(), None, None if sk is None else f64(sk), 0,
+                                        hd ** -0.5)
+    out[..., 5] = want[..., 5]
+    assert (np.abs(out - want) <= _attn_tol(dt, smax, vmax, want)).all()
