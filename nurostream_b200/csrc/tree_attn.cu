@@ -87,6 +87,13 @@ __device__ __forceinline__ float ta_row_scale(float m, float l, const float* sin
   return ex2(m - mm) / fmaf(l, ex2(m - mm), ex2(sk - mm - kTaShift<DT>));
 }
 
+// The maximum that a part of a row is stored with: -inf marks an unused node, whose row is zero.  A used one's is
+// finite or above even where the part has none (no key of it is seen, or every score is NaN or -inf; the
+// part's sum, zero or NaN, tells the rest).
+__device__ __forceinline__ float ta_part_max(bool used, float m) {
+  return used ? fmaxf(m, -3.402823466e38f) : -INFINITY;
+}
+
 // Keys [lo, hi) of sequence b that any node may see, and how many blocks they are.
 struct TaSpan {
   int lo, hi, len;
@@ -626,7 +633,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
           }
           const int row = at.rt * MR + r, t = row / a.rep, h = at.h * a.rep + row % a.rep;
           if (whole) {
-            const bool live = S.anc[t] != 0 && mt != -INFINITY;
+            const bool live = S.anc[t] != 0;  // a used node sees itself at least
             const float scale = live ? ta_row_scale<DT>(mt, lt, p.sinks, h) : 0.f;
             const int64_t oo = at.b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
 #pragma unroll
@@ -637,7 +644,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) po[lane + 32 * i] = acc[i];
             if (lane == 0) {
-              a.part_ml[((int64_t)slot * MR + r) * 2] = S.anc[t] ? mt : -INFINITY;
+              a.part_ml[((int64_t)slot * MR + r) * 2] = ta_part_max(S.anc[t] != 0, mt);
               a.part_ml[((int64_t)slot * MR + r) * 2 + 1] = lt;
             }
           }
@@ -650,7 +657,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
           if (r >= n_rows) continue;
           const int row = at.rt * MR + r, t = row / a.rep, h = at.h * a.rep + row % a.rep;
           if (whole) {
-            const bool live = anc[i] != 0 && m[i] != -INFINITY;
+            const bool live = anc[i] != 0;
             const float scale = live ? ta_row_scale<DT>(m[i], l[i], p.sinks, h) : 0.f;
             const int64_t oo = at.b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
 #pragma unroll
@@ -666,7 +673,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
             for (int n = 0; n < HD / 8; ++n)
               *reinterpret_cast<float2*>(po + n * 8 + 2 * tq) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
             if (tq == 0) {
-              a.part_ml[((int64_t)slot * MR + r) * 2] = anc[i] ? m[i] : -INFINITY;
+              a.part_ml[((int64_t)slot * MR + r) * 2] = ta_part_max(anc[i] != 0, m[i]);
               a.part_ml[((int64_t)slot * MR + r) * 2 + 1] = l[i];
             }
           }
@@ -725,7 +732,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const _
 
   auto finish = [&](int r, float mt, float lt, float (&acc)[V]) {  // one row out
     const int row = rt * MR + r, t = row / a.rep, h = hk * a.rep + row % a.rep;
-    const bool live = mt != -INFINITY;  // an unused node's parts say -inf
+    const bool live = mt != -INFINITY;  // only an unused node's parts all say so (ta_part_max)
     const float scale = live ? ta_row_scale<DT>(mt, lt, p.sinks, h) : 0.f;
     const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2] + lane * V;
 #pragma unroll

@@ -510,12 +510,12 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
         f0 = ex2(ma - ref), f1 = ex2(mb - ref);
         l = ml[128 + row] * f0 + ml[384 + row] * f1;
       }
-      const bool whole = it.n == it.pos.nblk, live = used && m != -INFINITY;
-      const float scale = whole && live ? ta_row_scale<DT>(m, l, p.sinks, h) : 0.f;
+      const bool whole = it.n == it.pos.nblk;
+      const float scale = whole && used ? ta_row_scale<DT>(m, l, p.sinks, h) : 0.f;
       const int slot = 2 * blockIdx.x + (u - it.pos.blk <= u0 ? 0 : 1);
       const int64_t pr = (int64_t)slot * MR + (PAIR ? s * 128 : 0) + row;
       const int64_t oo = b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
-      if (!whole && has_row && (PAIR || s == 0)) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(used ? m : -INFINITY, l);
+      if (!whole && has_row && (PAIR || s == 0)) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(ta_part_max(used, m), l);
       constexpr int NC = HD / 32;
 #pragma unroll 1
       for (int c = PAIR ? 0 : s * (NC / 2); c < (PAIR ? NC : (s + 1) * (NC / 2)); ++c) {
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
             if (32 * c + i < p.head_dim) {
               float y[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) y[k] = live ? o[i + k] * scale : 0.f;
+              for (int k = 0; k < 8; ++k) y[k] = used ? o[i + k] * scale : 0.f;
               if (a.vec & 2) {
                 store8(p.out, DT, oo + 32 * c + i, y);
               } else {

@@ -693,3 +693,45 @@ def test_attention_sums_of_large_values(T, hq, hkv, hd, sinks, dt):
                                         hd ** -0.5)
     out[..., 5] = want[..., 5]
     assert (np.abs(out - want) <= _attn_tol(dt, smax, vmax, want)).all()
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("B,T,hq,hkv,hd,n", [
+    (1, 1, 2, 2, 64, 0),          # nothing but itself
+    (1, 1, 8, 1, 128, 2000),      # one token, cut into many parts that several warps join
+    (2, 6, 8, 2, 64, 700),        # one slot of rows, cut
+    (60, 6, 8, 2, 64, 40),        # whole items
+    (2, 40, 16, 4, 64, 900),      # two slots of rows, cut
+    (30, 40, 16, 4, 128, 60),
+    (4, 64, 32, 2, 64, 1500),     # parts that a warp joins alone, several tiles of rows
+])
+def test_a_nan_query_gives_nan(B, T, hq, hkv, hd, n, sinks, dt):
+    """In its own row alone, whatever type, number of rows or cut."""
+    q, kc, vc, lens, par, sk = _attn_case(B, T, hq, hkv, hd, n, T > 1, sinks, dt)
+    base = spec.tree_attention(q, kc, vc, lens, par, sinks=sk)
+    rows = {(b, t, h) for b in range(0, B, 2) for t, h in ((0, 0), (T // 2, hq - 1), (T - 1, hq // 2))}
+    for b, t, h in rows:
+        if dt == F32:
+            _put(q[b, t, h, 1], "nan")
+        else:
+            q[b, t, h, 1] = float("nan")
+    out = spec.tree_attention(q, kc, vc, lens, par, sinks=sk)
+    for b, t, h in rows:
+        if par is not None and par[b, t] == -2:
+            assert not out[b, t, h].any()
+        else:
+            assert torch.isnan(out[b, t, h]).all(), (b, t, h)
+        out[b, t, h] = base[b, t, h]
+    assert torch.equal(out, base)
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("T,hq,hkv,hd", [(1, 2, 1, 64), (1, 8, 2, 128), (7, 8, 2, 64), (33, 16, 2, 64)])
+def test_scores_of_minus_infinity_alone(T, hq, hkv, hd, dt):
+    """Every seen score -inf: the softmax has nothing to divide by, unless a sink gives it something."""
+    q, kc, vc, lens, _, _ = _attn_case(1, T, hq, hkv, hd, 300, False, False, dt)
+    q[..., 0], kc[..., 0] = q[..., 0].abs() + 0.1, float("-inf")
+    assert torch.isnan(spec.tree_attention(q, kc, vc, lens)).all()
+    sk = torch.zeros(hq, device="cuda")
+    assert not spec.tree_attention(q, kc, vc, lens, sinks=sk).any()
