@@ -373,6 +373,11 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
     const int k0 = sp.lo + at.blk * BN;
     // a block needs no mask when every row sees all of it
     const bool masked = k0 + BN > sp.len || (p.window > 0 && sp.len + S.max_depth - k0 >= p.window);
+    auto sees = [&](int i, int key) {  // whether this thread's row i sees a key of the item
+      if (key < sp.len) return anc[i] != 0 && (p.window == 0 || sp.len + dep[i] - key < p.window);
+      const int nd = key - sp.len;
+      return nd < p.T && nd < kTreeMax && (anc[i] >> nd & 1) && (p.window == 0 || dep[i] - S.depth[nd] < p.window);
+    };
     // Values that not every row sees may hold anything, and fp32 products take no infinities: rows of the block that
     // hold such values are set to zero here and added, for the rows that see them, from the cache below.
     const bool look = DT == NS_F32 || masked;
@@ -442,16 +447,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
         for (int n = 0; n < SB / 8; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int key = k0 + kr + n * 8 + 2 * tq + (j & 1), i = j >> 1;
-            bool see;
-            if (key < sp.len) {
-              see = anc[i] != 0 && (p.window == 0 || sp.len + dep[i] - key < p.window);
-            } else {
-              const int nd = key - sp.len;
-              see = nd < p.T && nd < kTreeMax && (anc[i] >> nd & 1) &&
-                    (p.window == 0 || dep[i] - S.depth[nd] < p.window);
-            }
-            if (!see) s[n][j] = -INFINITY;
+            if (!sees(j >> 1, k0 + kr + n * 8 + 2 * tq + (j & 1))) s[n][j] = -INFINITY;
           }
       }
       if constexpr (DT == NS_F32) {  // scores that came out as NaN: the products may not have taken q or k
@@ -571,6 +567,8 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
           const int from = (lane & ~3) | ((kk & 7) >> 1);
           pv[0] = __shfl_sync(0xffffffffu, pv[0], from);
           pv[1] = __shfl_sync(0xffffffffu, pv[1], from);
+          // (by the mask: a probability may be too small for its type and the value still count)
+          const bool see[2] = {sees(0, k0 + kr + kk), sees(1, k0 + kr + kk)};
           const int64_t vrow = at.b * p.vc_stride[0] + at.h * p.vc_stride[1] + (int64_t)(k0 + kr + kk) * p.vc_stride[2];
 #pragma unroll
           for (int n = 0; n < HD / 8; ++n)
@@ -579,8 +577,8 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
               const int d = n * 8 + 2 * tq + j;
               if (d >= p.head_dim) continue;
               const float v = load_float(p.v_cache, DT, vrow + d);
-              if (pv[0] != 0.f) o[n][j] = fmaf(pv[0], v, o[n][j]);
-              if (pv[1] != 0.f) o[n][2 + j] = fmaf(pv[1], v, o[n][2 + j]);
+              if (see[0]) o[n][j] = fmaf(pv[0], v, o[n][j]);
+              if (see[1]) o[n][2 + j] = fmaf(pv[1], v, o[n][2 + j]);
             }
           __syncwarp();  // the products of the next keys are .aligned
         }
@@ -817,19 +815,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const _
 #pragma unroll
       for (int j = 0; j < V; ++j) acc[j] *= f;
       const int m = min(32, to - c);
-      for (int i = 0; i < m; i += 4) {  // four parts in flight; past the end the last one again, with weight zero
+      for (int i = 0; i < m; i += 4) {  // four parts in flight; past the end the last one again, not added
         float v[4][V], w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int src = min(i + k, m - 1);
           w[k] = __shfl_sync(0xffffffffu, fi, src);
-          if (i + k >= m) w[k] = 0.f;
           load_part(__shfl_sync(0xffffffffu, base, src), v[k]);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int j = 0; j < V; ++j) acc[j] = w[k] != 0.f ? fmaf(v[k][j], w[k], acc[j]) : acc[j];
+          for (int j = 0; j < V; ++j) acc[j] = i + k < m ? fmaf(v[k][j], w[k], acc[j]) : acc[j];
       }
     }
 #pragma unroll
@@ -849,7 +846,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const _
         const float f = ex2(sm[w] - ref);
         lt = fmaf(sl[w], f, lt);
 #pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] = f != 0.f ? fmaf(so[w][lane * V + j], f, acc[j]) : acc[j];
+        for (int j = 0; j < V; ++j) acc[j] = fmaf(so[w][lane * V + j], f, acc[j]);
       }
       finish(r0, mt, lt, acc);
     }

@@ -470,6 +470,8 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
               asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n tcgen05.wait::ld.sync.aligned;"
                            : "=r"(w) : "r"(s_col(s) + lane_base + (kk >> 1)) : "memory");
               w = kk & 1 ? w >> 16 : w & 0xFFFFu;
+              const int nd = k0 + kk - sp.len;
+              const bool see = nd < 0 ? k0 + kk >= klo : nd < kTreeMax && (vis >> nd & 1);
               const float pv = DT == NS_F16 ? f16_bits_to_float(w) : __uint_as_float(w << 16);
               const int64_t vrow = b * p.vc_stride[0] + it.pos.h * p.vc_stride[1] + (int64_t)(k0 + kk) * p.vc_stride[2];
 #pragma unroll 1
@@ -479,7 +481,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1) tree_attn_tc_kernel(const _
                 tmem_wait_ld_x32(o);
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                  if (pv != 0.f && 32 * c + i < p.head_dim) o[i] = fmaf(pv, load_float(p.v_cache, DT, vrow + 32 * c + i), o[i]);
+                  if (see && 32 * c + i < p.head_dim) o[i] = fmaf(pv, load_float(p.v_cache, DT, vrow + 32 * c + i), o[i]);
                 __syncwarp();  // lanes whose row does not see the key skipped the loads
                 tmem_st_x32(o_col(s) + lane_base + 32 * c, reinterpret_cast<const uint32_t*>(o));
               }

@@ -735,3 +735,20 @@ def test_scores_of_minus_infinity_alone(T, hq, hkv, hd, dt):
     assert torch.isnan(spec.tree_attention(q, kc, vc, lens)).all()
     sk = torch.zeros(hq, device="cuda")
     assert not spec.tree_attention(q, kc, vc, lens, sinks=sk).any()
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("T,hq,hkv,hd", [(1, 2, 2, 64), (1, 16, 2, 128), (7, 8, 2, 64), (9, 32, 2, 64), (40, 16, 2, 128)])
+@pytest.mark.parametrize("key", [10, 1200, 1997])
+def test_a_seen_nan_value_counts_however_small_its_probability(T, hq, hkv, hd, key, dt):
+    """Zero in the type, or the whole part's weight zero: zero times NaN is NaN, in a masked block and an open one, in
+    parts that are joined by a warp each and by several."""
+    n, rep = 2000, hq // hkv
+    q, kc, vc, lens, _, _ = _attn_case(1, T, hq, hkv, hd, n, False, False, dt)
+    q[..., 0], kc[..., 0] = 64.0, 20.0
+    kc[:, :, :300, 0], kc[:, :, key, 0] = -20.0, -20.0
+    base = spec.tree_attention(q, kc, vc, lens)
+    assert torch.isfinite(base).all()
+    vc[0, 0, key] = float("nan")
+    out = spec.tree_attention(q, kc, vc, lens)
+    assert torch.isnan(out[:, :, :rep]).all() and torch.equal(out[:, :, rep:], base[:, :, rep:])
