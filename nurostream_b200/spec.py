@@ -59,6 +59,7 @@ _LAYOUTS: dict = {}
 _LAST: dict = {}
 _MAX_LAYOUTS = 4096
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _sig(t: torch.Tensor | None):
@@ -85,6 +86,16 @@ def _keep(key, layout):
 
 def _stream(t: torch.Tensor) -> int:
     return _raw_stream(t.get_device()) if _raw_stream is not None else torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _launch(t: torch.Tensor, name: str, *args) -> None:
+    """Entry point ``name`` on the device of t and its current stream; the library launches on the current device."""
+    device = t.get_device()
+    if device == _current_device():
+        _lib.call(name, *args, _stream(t))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _stream(t))
 
 
 def _ptr(t: torch.Tensor | None):
@@ -177,7 +188,7 @@ def _rope_call(q, k, v, q_out, kc, vc, cos, sin, lens, parents, positions, rotar
     p.q, p.q_out = q.data_ptr(), q_out.data_ptr()
     if kc is not None:
         p.k, p.v, p.k_cache, p.v_cache = k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr()
-    _lib.call("ns_rope_append", C.byref(p), _stream(q))
+    _launch(q, "ns_rope_append", C.byref(p))
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -258,7 +269,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     p.lens, p.parents, p.sinks = lens.data_ptr(), _ptr(parents), _ptr(sinks)
     p.q, p.k_cache, p.v_cache, p.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr()
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-    _lib.call("ns_tree_attn", C.byref(p), ws.data_ptr(), ws_bytes, _stream(q))
+    _launch(q, "ns_tree_attn", C.byref(p), ws.data_ptr(), ws_bytes)
     return o
 
 
@@ -310,7 +321,7 @@ def verify_tree(tokens: torch.Tensor, logits: torch.Tensor, uniforms: torch.Tens
     p.tokens, p.logits, p.uniforms, p.race = tokens.data_ptr(), logits.data_ptr(), uniforms.data_ptr(), race.data_ptr()
     p.parents, p.draft_probs, p.temperature = _ptr(parents), _ptr(draft_probs), _ptr(temperature)
     p.path, p.n_accepted, p.next_token = path.data_ptr(), n_acc.data_ptr(), nxt.data_ptr()
-    _lib.call("ns_tree_verify", C.byref(p), _stream(logits))
+    _launch(logits, "ns_tree_verify", C.byref(p))
     return path, n_acc, nxt
 
 
@@ -361,5 +372,5 @@ def commit_path(caches, lens: torch.Tensor, path: torch.Tensor, n_accepted: torc
     p.lens, p.path, p.n_accepted, p.new_lens = lens.data_ptr(), path.data_ptr(), n_accepted.data_ptr(), out.data_ptr()
     ptr = torch.Tensor.data_ptr
     p.k_cache[:n], p.v_cache[:n] = list(map(ptr, ks)), list(map(ptr, vs))
-    _lib.call("ns_path_commit", C.byref(p), _stream(k0))
+    _launch(k0, "ns_path_commit", C.byref(p))
     return out

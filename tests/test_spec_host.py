@@ -1,0 +1,68 @@
+"""Host side of nurostream_b200.spec without a GPU: on which device and stream the operators launch."""
+import contextlib
+
+import pytest
+import torch
+
+from nurostream_b200 import spec
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that says it is on cuda:1 (its pointer is never used: the entry points are replaced)."""
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        kwargs = dict(kwargs or {})
+        if "device" in kwargs:
+            kwargs["device"] = "cpu"
+        out = super().__torch_function__(func, types, args, kwargs)
+        return out
+
+    device = property(lambda self: torch.device("cuda", 1))
+    is_cuda = property(lambda self: True)
+
+    def get_device(self):
+        return 1
+
+
+def _on(*shape, dtype=torch.float32):
+    return torch.zeros(shape, dtype=dtype).as_subclass(OnDevice)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Entry points that were called, with the device that was current and the stream they got."""
+    seen, current = [], [0]
+
+    @contextlib.contextmanager
+    def device(i):
+        before, current[0] = current[0], i
+        yield
+        current[0] = before
+
+    def empty(*args, device=None, **kw):
+        return torch.zeros(*args, **kw).as_subclass(OnDevice)
+
+    monkeypatch.setattr(spec, "_current_device", lambda: current[0], raising=False)
+    monkeypatch.setattr(spec, "_raw_stream", lambda i: 1000 + i)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch, "empty", empty)
+    monkeypatch.setattr(spec._lib, "call", lambda name, *args: seen.append((name, current[0], args[-1])))
+    monkeypatch.setattr(spec, "_LAYOUTS", {})
+    monkeypatch.setattr(spec, "_LAST", {})
+    yield seen
+    assert current == [0]
+
+
+def test_operators_launch_on_the_device_of_their_tensors(calls):
+    """Tensors on cuda:1 while cuda:0 is current: the launch has to be made on cuda:1, on a stream of it."""
+    i32 = torch.int32
+    q, kv, cache, lens = _on(1, 2, 4, 64), _on(1, 2, 2, 64), _on(1, 2, 8, 64), _on(1, dtype=i32)
+    table, tokens, path = _on(8, 32), _on(1, 2, dtype=i32), _on(1, 2, dtype=i32)
+    spec.rope_append(q, kv, kv, table, table, cache, cache, lens)
+    spec.tree_attention(q, cache, cache, lens)
+    spec.verify_tree(tokens, _on(1, 2, 9), _on(1, 2), _on(1, 9))
+    spec.commit_path([(cache, cache)], lens, path, lens, new_lens=_on(1, dtype=i32))
+    launches = [c for c in calls if c[0] != "ns_tree_attn_workspace_bytes"]
+    assert [c[0] for c in launches] == ["ns_rope_append", "ns_tree_attn", "ns_tree_verify", "ns_path_commit"]
+    assert all(c[1:] == (1, 1001) for c in launches)
