@@ -367,8 +367,9 @@ class SpecDecoder:
     lookup in the text so far).  Per layer: the decoder's q/k/v projection of every node, ``spec.rope_append``,
     ``spec.tree_attention``, the output projection, and the MoE layer over all nodes (``prefill_grouped``);
     then the LM head, ``spec.verify_tree`` and ``spec.commit_path``.  The context length lives in
-    ``self.lens`` on the device and advances by the accepted nodes; plain ``decoder.step`` calls may follow at
-    that position.  One rank (world 1); a chain (parents None) or a tree of at most ``spec.MAX_NODES`` nodes.
+    ``self.lens`` on the device, always the same tensor, and advances by the accepted nodes; plain
+    ``decoder.step`` calls may follow at that position.  A step may be captured into a CUDA graph, after one
+    outside it (workspaces), and replayed: it reads its inputs and ``self.lens`` anew.  One rank (world 1); a chain (parents None) or a tree of at most ``spec.MAX_NODES`` nodes.
     """
 
     def __init__(self, decoder: GptOssDecoder, n_nodes: int):
@@ -381,6 +382,7 @@ class SpecDecoder:
         sh, dev, T = decoder.shape, decoder.device, n_nodes
         f32 = dict(dtype=torch.float32, device=dev)
         self.lens = torch.full((1,), decoder.ctx, dtype=torch.int32, device=dev)
+        self._new_lens = torch.empty_like(self.lens)
         self.tokens = torch.zeros((1, T), dtype=torch.int32, device=dev)
         self.xs = [torch.empty((T, sh.n_embd), **f32) for _ in range(3)]
         self.qkv = torch.empty((T, sh.q_dim + 2 * sh.kv_dim), **f32)
@@ -427,5 +429,5 @@ class SpecDecoder:
         logits = self.forward(tokens, parents)
         path, n_acc, token = self._spec.verify_tree(self.tokens, logits, uniforms, race, parents, draft_probs=draft_probs,
                                                     temperature=temperature)
-        self.lens = self._spec.commit_path(self.caches, self.lens, path, n_acc)
+        self.lens.copy_(self._spec.commit_path(self.caches, self.lens, path, n_acc, new_lens=self._new_lens))
         return path, n_acc, token

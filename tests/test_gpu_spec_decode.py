@@ -83,6 +83,35 @@ def test_one_node_is_a_plain_step():
         assert int(n) == 0 and int(nxt) == toks[i + 1] and int(s.lens) == CTX + i + 1
 
 
+def test_a_captured_step_goes_on_from_the_context_it_left():
+    """Replays of one graph, with other drafts each time, against plain decoding token by token."""
+    T = 4
+    toks, rows = _greedy(12)
+    s = SpecDecoder(_decoder(), T)
+    tokens, parents = _ints([[0] * T]), _ints([[-1, 0, 1, 1]])
+    u, race, greedy = torch.rand(1, T, device="cuda"), torch.ones(1, 512, device="cuda"), torch.zeros(1, device="cuda")
+    s.step(tokens, u, race, parents, temperature=greedy)     # workspaces
+    s.lens.fill_(CTX)
+    lens = s.lens
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        path, n, nxt = s.step(tokens, u, race, parents, temperature=greedy)
+    assert s.lens is lens and int(lens) == CTX               # captured, not run
+    at = 0
+    for right in (2, 0, 1, 2):                               # drafts that plain decoding would have taken
+        draft = [toks[at]] + [toks[at + 1 + i] if i < right else (toks[at + 1 + i] + 7) % 512 for i in range(2)]
+        tokens.copy_(_ints([draft + [(toks[at + 2] + 9) % 512]]))
+        graph.replay()
+        assert int(n) == right and int(nxt) == toks[at + right + 1] and path[0, :right + 1].tolist() == list(range(right + 1))
+        for i in range(right + 1):
+            _close(s.logits[0, i], rows[at + i])
+        at += right + 1
+        assert int(s.lens) == CTX + at
+    s.dec.set_token(toks[at], CTX + at)
+    _close(s.dec.step(), rows[at])
+    assert _lib.device_error() == 0
+
+
 def test_refusals():
     dec = _decoder()
     for n in (0, 65):
