@@ -383,6 +383,8 @@ class SpecDecoder:
         f32 = dict(dtype=torch.float32, device=dev)
         self.lens = torch.full((1,), decoder.ctx, dtype=torch.int32, device=dev)
         self._new_lens = torch.empty_like(self.lens)
+        self._node = torch.arange(n_nodes, dtype=torch.int32, device=dev)
+        self._chain = (self._node - 1)[None]
         self.tokens = torch.zeros((1, T), dtype=torch.int32, device=dev)
         self.xs = [torch.empty((T, sh.n_embd), **f32) for _ in range(3)]
         self.qkv = torch.empty((T, sh.q_dim + 2 * sh.kv_dim), **f32)
@@ -425,7 +427,14 @@ class SpecDecoder:
     def step(self, tokens: torch.Tensor, uniforms: torch.Tensor, race: torch.Tensor, parents: torch.Tensor | None = None,
              draft_probs: torch.Tensor | None = None, temperature: torch.Tensor | None = None):
         """One speculative step: (path, n_accepted, next_token) as ``spec.verify_tree`` gives them, the accepted
-        nodes' keys and values in place and ``self.lens`` advanced past them.  No host synchronisation."""
+        nodes' keys and values in place and ``self.lens`` advanced past them.  No host synchronisation.
+
+        Nodes that the cache has no slot for (lens + t >= max_ctx) count as unused and are not accepted.  Once not even
+        node 0 has one, nothing moves: next_token is -1, the path empty, and the device's error word says so."""
+        parents = self._chain if parents is None else parents
+        if tuple(parents.shape) != (1, self.n_nodes):
+            raise ValueError(f"parents has shape {tuple(parents.shape)}; expected {(1, self.n_nodes)}")
+        parents = torch.where(self.lens + self._node < self.dec.max_ctx, parents, -2)
         logits = self.forward(tokens, parents)
         path, n_acc, token = self._spec.verify_tree(self.tokens, logits, uniforms, race, parents, draft_probs=draft_probs,
                                                     temperature=temperature)

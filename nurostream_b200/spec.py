@@ -307,6 +307,8 @@ def verify_tree(tokens: torch.Tensor, logits: torch.Tensor, uniforms: torch.Tens
     uniforms[c] * q(c) < r(c), with r the target's distribution less the drafts rejected before it; the tokens
     that come out are distributed as the target's own.  path (B, T): accepted nodes from node 0 on, then -1;
     n_accepted (B) drafts; next_token (B), drawn as the largest r / race (-1 if a row's logits are all -inf).
+    The cache is not known here: nodes without a slot in it (lens + t >= max_ctx) have to be marked unused in
+    ``parents`` (as ``gptoss.SpecDecoder.step`` does), or they may be accepted on logits that saw nothing.
     """
     key = ("verify", _sig(tokens), _sig(logits), _sig(uniforms), _sig(race), _sig(parents), _sig(draft_probs),
            _sig(temperature))

@@ -112,8 +112,42 @@ def test_a_captured_step_goes_on_from_the_context_it_left():
     assert _lib.device_error() == 0
 
 
+@pytest.mark.parametrize("tree", [False, True])
+def test_nodes_past_the_end_of_the_cache_are_not_accepted(tree):
+    """Three slots left for six nodes that plain decoding would all have taken; then none."""
+    full = 128
+
+    def decoder():
+        return GptOssDecoder(GptOssShape(**SHAPE), torch.device("cuda", 0), seed=3, ctx=full - 3, max_ctx=full)
+
+    dec, toks, rows = decoder(), [5], []
+    for i in range(3):
+        dec.set_token(toks[-1], full - 3 + i)
+        rows.append(dec.step().clone())
+        toks.append(int(rows[-1].argmax()))
+    s = SpecDecoder(decoder(), 6)
+    u, race, greedy = torch.rand(1, 6, device="cuda"), torch.ones(1, 512, device="cuda"), torch.zeros(1, device="cuda")
+    parents = _ints([[-1, 0, 1, 2, 2, 3]]) if tree else None
+    tokens = [t % 512 for t in (toks[0], toks[1], toks[2], toks[3], toks[3], toks[3])]
+    path, n, nxt = s.step(_ints(tokens), u, race, parents, temperature=greedy)
+    assert path.tolist() == [[0, 1, 2, -1, -1, -1]] and int(n) == 2 and int(nxt) == toks[3] and int(s.lens) == full
+    for i in range(3):
+        _close(s.logits[0, i], rows[i])
+    assert _lib.device_error() == 0
+    caches = [c.clone() for kv in s.caches for c in kv]
+    path, n, nxt = s.step(_ints(tokens), u, race, parents, temperature=greedy)
+    assert path.tolist() == [[-1] * 6] and int(n) == 0 and int(nxt) == -1 and int(s.lens) == full
+    assert _lib.device_error() & _lib.DEVERR_ROUTE
+    assert all(torch.equal(a, b) for a, b in zip(caches, (c for kv in s.caches for c in kv)))
+
+
 def test_refusals():
     dec = _decoder()
     for n in (0, 65):
         with pytest.raises(ValueError):
             SpecDecoder(dec, n)
+    s = SpecDecoder(dec, 3)
+    u, race = torch.rand(1, 3, device="cuda"), torch.ones(1, 512, device="cuda")
+    for bad in ([[-1]], [[-1, 0, 1, 2]], [-1, 0, 1]):
+        with pytest.raises(ValueError):
+            s.step(_ints([1, 2, 3]), u, race, _ints(bad))
