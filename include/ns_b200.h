@@ -479,7 +479,7 @@ int ns_tree_attn(const ns_tree_attn_t* p, void* workspace, size_t workspace_byte
  * largest logit (lowest index on ties), a child is accepted if it is that token,
  * and it is the next token.  A NaN logit counts as -inf, +inf as the largest
  * finite number; a row of nothing else than -inf accepts nothing and gives token -1.
- * At most 1024 nodes and a vocabulary of 204800.
+ * At most 1024 nodes and a vocabulary of 204800.  A token outside the vocabulary is never accepted.
  * Results: path (B x T: accepted nodes from node 0 on, then -1), n_accepted (B:
  * accepted nodes, node 0 not counted), next_token (B).
  */

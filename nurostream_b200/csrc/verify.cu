@@ -183,6 +183,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) tree_verify_kernel(const __
     }
     s_kid[t] = (int16_t)kid;
     s_sib[t] = (int16_t)sib;
+    // a parent out of order, below -2 or unused: the walk never comes to the node, but the tree is wrong
+    const int up = s_par[t];
+    if (rank == 0 && (up >= t || up < -2 || (up >= 0 && s_par[up] == -2))) raise_device_error(NS_DEVERR_ROUTE);
   }
   __syncthreads();
   const bool root_ok = s_par[0] == -1;

@@ -752,3 +752,21 @@ def test_a_seen_nan_value_counts_however_small_its_probability(T, hq, hkv, hd, k
     vc[0, 0, key] = float("nan")
     out = spec.tree_attention(q, kc, vc, lens)
     assert torch.isnan(out[:, :, :rep]).all() and torch.equal(out[:, :, rep:], base[:, :, rep:])
+
+
+@pytest.mark.parametrize("parents", [[-1, 0, 2, 0, -2], [-1, 0, 3, 0, -2], [-1, 0, -3, 0, -2], [-1, 0, 0, -2, 3]])
+def test_verify_flags_a_bad_parent(parents):
+    """Itself, a later node, no parent at all, an unused one: flagged, never accepted, and the rest of the tree stands."""
+    z = torch.full((2, 5, 300), -9.0, device="cuda")
+    tokens = _ints([[1, 2, 3, 4, 5]] * 2)
+    good = [-1, 0, 1, -2, -2]                        # the other sequence
+    z[0, 0, 2], z[0, 1, 3] = 9.0, 9.0                # node 1 is right; node 2 would be, below it
+    z[1, 0, 2], z[1, 1, 3], z[1, 2, 7] = 9.0, 9.0, 9.0
+    u, race = torch.full((2, 5), 0.5, device="cuda"), torch.ones(2, 300, device="cuda")
+    for temp in (None, torch.zeros(2, device="cuda")):
+        path, n, nxt = spec.verify_tree(tokens, z, u, race, _ints([parents, good]), temperature=temp)
+        assert _errors()
+        assert path.tolist() == [[0, 1, -1, -1, -1], [0, 1, 2, -1, -1]]
+        assert n.tolist() == [1, 2] and nxt.tolist() == [3, 7]
+    spec.verify_tree(tokens, z, u, race, _ints([good, good]))
+    assert not _errors()
