@@ -475,7 +475,7 @@ int ns_tree_attn(const ns_tree_attn_t* p, void* workspace, size_t workspace_byte
  *   r = normalise(max(r - q, 0)) (kept if nothing is left), q(c) = 0, q renormalised.
  * When no child is accepted, the next token is drawn from r: the index with the
  * largest r(x) / race[x], race holding draws of Exp(1).  The tokens emitted this
- * way are distributed as the target's own.  temperature[b] = 0: r is all on the
+ * way are distributed as the target's own.  Temperatures are finite and at least 0.  temperature[b] = 0: r is all on the
  * largest logit (lowest index on ties), a child is accepted if it is that token,
  * and it is the next token.  A NaN logit counts as -inf, +inf as the largest
  * finite number; a row of nothing else than -inf accepts nothing and gives token -1.

@@ -172,8 +172,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) tree_verify_kernel(const __
   }
   const float temp = p.temperature ? p.temperature[b] : 1.f;
   const bool greedy = temp == 0.f;
-  // exp(x / temperature) = 2^(c x)
-  const float cf = greedy ? 1.f : 1.4426950408889634f / temp;
+  // exp(x / temperature) = 2^(c x), c finite: a subnormal temperature would make it infinite, and the maximum's
+  // own distance of zero NaN
+  const float cf = greedy ? 1.f : 1.4426950408889634f / fmaxf(temp, 1.17549435e-38f);
   __syncthreads();
   for (int t = tid; t < p.T; t += kVerifyThreads) {  // the tree as lists of children in node order
     int kid = -1, sib = -1;

@@ -303,7 +303,7 @@ def verify_tree(tokens: torch.Tensor, logits: torch.Tensor, uniforms: torch.Tens
     tokens (B, T) int32; logits (B, T, V) the target's, after each node; draft_probs (B, T, V): the distribution that
     each node's children were drawn from, without replacement, in node order (None: the drafts were certain, as those
     of a lookup or of a greedy draft); uniforms (B, T) in [0, 1) and race (B, V) draws of Exp(1), fp32: the random
-    numbers.  temperature (B,) fp32: 0 is greedy, None is 1.  From node 0 a child c is accepted if
+    numbers.  temperature (B,) fp32, finite: 0 is greedy, None is 1.  From node 0 a child c is accepted if
     uniforms[c] * q(c) < r(c), with r the target's distribution less the drafts rejected before it; the tokens
     that come out are distributed as the target's own.  path (B, T): accepted nodes from node 0 on, then -1;
     n_accepted (B) drafts; next_token (B), drawn as the largest r / race (-1 if a row's logits are all -inf).

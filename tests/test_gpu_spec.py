@@ -770,3 +770,15 @@ def test_verify_flags_a_bad_parent(parents):
         assert n.tolist() == [1, 2] and nxt.tolist() == [3, 7]
     spec.verify_tree(tokens, z, u, race, _ints([good, good]))
     assert not _errors()
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 4e-39, 1e-42, 1.4e-45])
+def test_verify_at_the_smallest_temperatures(temperature):
+    """Down to the last subnormal: all on the largest logit."""
+    tokens, z, u, race, par, d, _ = _verify_case(4, 9, 3001, True, True, F32, 5)
+    temp = torch.full((4,), temperature, device="cuda")
+    assert (temp > 0).all()
+    got = spec.verify_tree(tokens, z, u, race, par, draft_probs=d, temperature=temp)
+    want = spec.verify_tree(tokens, z, u, race, par, draft_probs=d, temperature=torch.zeros(4, device="cuda"))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
