@@ -63,6 +63,8 @@ extern "C" int ns_path_commit(const ns_path_commit_t* p, ns_stream_t stream) {
     return fail(NS_ERR_INVALID, "ns_path_commit: %d layers (at most %d)", p->n_layer, NS_COMMIT_MAX_LAYERS);
   if (p->B < 0 || p->T < 1 || p->n_head_kv < 1 || p->head_dim < 1 || p->max_ctx < 0)
     return fail(NS_ERR_INVALID, "ns_path_commit: bad B, T, head count, head_dim or max_ctx");
+  if (p->T > INT32_MAX - p->max_ctx)  // slots are counted in 32 bits
+    return fail(NS_ERR_UNSUPPORTED, "ns_path_commit: caches of %d slots, %d nodes", p->max_ctx, p->T);
   if (!float_type_ok(p->dtype)) return fail(NS_ERR_INVALID, "ns_path_commit: bad dtype %d", p->dtype);
   if (p->B > 65535) return fail(NS_ERR_UNSUPPORTED, "ns_path_commit: %d sequences (at most 65535)", p->B);
   if (p->B == 0) return NS_OK;

@@ -934,6 +934,8 @@ static int ta_check(const ns_tree_attn_t* p) {
   if (!p) return fail(NS_ERR_INVALID, "ns_tree_attn: null parameters");
   if (p->B < 0 || p->T < 0 || p->max_ctx < 1 || p->window < 0)
     return fail(NS_ERR_INVALID, "ns_tree_attn: B %d, T %d, max_ctx %d, window %d", p->B, p->T, p->max_ctx, p->window);
+  // slots are counted in 32 bits, up to the nodes and a block past the last one
+  if (p->max_ctx > INT32_MAX - 1024) return fail(NS_ERR_UNSUPPORTED, "ns_tree_attn: caches of %d slots", p->max_ctx);
   if (!float_type_ok(p->dtype)) return fail(NS_ERR_INVALID, "ns_tree_attn: bad dtype %d", p->dtype);
   if (p->T > NS_TREE_MAX_NODES)
     return fail(NS_ERR_UNSUPPORTED, "ns_tree_attn: %d nodes (at most %d)", p->T, NS_TREE_MAX_NODES);

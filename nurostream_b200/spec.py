@@ -36,6 +36,8 @@ def _rows(name: str, t: torch.Tensor, shape: tuple, dev) -> None:
     """t: a CUDA tensor of this shape whose innermost dimension is contiguous (the others may be strided)."""
     if tuple(t.shape) != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}; expected {shape}")
+    if max(shape, default=0) > 0x7FFFFFFF:
+        raise ValueError(f"{name} has a dimension of more than 2^31 - 1: {shape}")
     if t.device != dev or not t.is_cuda:
         raise ValueError(f"{name} is on {t.device}; expected {dev} (a CUDA device, no CPU fallback)")
     if t.stride(-1) != 1 and t.shape[-1] > 1:

@@ -147,3 +147,15 @@ def test_rope_refuses_tables_without_rows(lib):
     assert lib.ns_rope_append(C.byref(_rope(n_pos=0)), None) == -1
     assert b"tables without rows" in lib.ns_last_error()
     assert lib.ns_rope_append(C.byref(_rope(n_pos=0, T=0)), None) == 0
+
+
+def test_caches_of_more_slots_than_are_counted(lib):
+    """Slots, nodes and a block past them are counted in 32 bits."""
+    top = 2 ** 31 - 1
+    n = C.c_size_t(0)
+    assert lib.ns_tree_attn_workspace_bytes(C.byref(_attn(max_ctx=top)), C.byref(n)) == -2
+    assert lib.ns_tree_attn(C.byref(_attn(max_ctx=top)), 256, 1 << 30, None) == -2
+    assert lib.ns_tree_attn_workspace_bytes(C.byref(_attn(max_ctx=top - 1024)), C.byref(n)) == 0
+    assert lib.ns_path_commit(C.byref(_commit(max_ctx=top, B=0)), None) == -2
+    assert lib.ns_path_commit(C.byref(_commit(max_ctx=top - 3, B=0)), None) == -2
+    assert lib.ns_path_commit(C.byref(_commit(max_ctx=top - 4, B=0)), None) == 0

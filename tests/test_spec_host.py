@@ -66,3 +66,10 @@ def test_operators_launch_on_the_device_of_their_tensors(calls):
     launches = [c for c in calls if c[0] != "ns_tree_attn_workspace_bytes"]
     assert [c[0] for c in launches] == ["ns_rope_append", "ns_tree_attn", "ns_tree_verify", "ns_path_commit"]
     assert all(c[1:] == (1, 1001) for c in launches)
+
+
+def test_dimensions_that_the_library_cannot_count(calls):
+    """They would arrive there modulo 2^32."""
+    cache = torch.zeros(1, 1, 1, 8, dtype=torch.float16).expand(1, 1, 2 ** 32 + 5, 8).as_subclass(OnDevice)
+    with pytest.raises(ValueError, match="dimension"):
+        spec.tree_attention(_on(1, 2, 1, 8, dtype=torch.float16), cache, cache, _on(1, dtype=torch.int32))
