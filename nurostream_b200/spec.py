@@ -141,7 +141,9 @@ def rope_tables(rotary_dim: int, n_pos: int, base: float = 10000.0, scaling: str
 
 
 def _rope_layout(q, k, v, q_out, kc, vc, cos, sin, lens, parents, positions, rotary_dim, interleaved):
-    """Checks of a rope call (k, v and the caches may be None) and its parameter block without pointers."""
+    """Checks of a rope call (k, v and the caches may be None together) and its parameter block without pointers."""
+    if len({t is None for t in (k, v, kc, vc)}) > 1:
+        raise TypeError("k, v, k_cache and v_cache are given together")
     if q.dim() != 4 or (kc is not None and kc.dim() != 4):
         raise ValueError("q must be (B, T, n_head, hd) and the caches (B, n_head_kv, max_ctx, hd)")
     B, T, hq, hd = q.shape
@@ -207,6 +209,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     ``interleaved``.  q_out may be q (in place).  Rows of unused nodes: zero in q_out, nothing in the cache.
     With parents, T <= MAX_NODES; a chain (parents None) may have any T (a prompt).
     """
+    if k is None:
+        raise TypeError("k and v are missing (rope rotates without a cache)")
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
     _rope_call(q, k, v, out, k_cache, v_cache, cos, sin, lens, parents, positions, rotary_dim, interleaved)
     return out

@@ -73,3 +73,13 @@ def test_dimensions_that_the_library_cannot_count(calls):
     cache = torch.zeros(1, 1, 1, 8, dtype=torch.float16).expand(1, 1, 2 ** 32 + 5, 8).as_subclass(OnDevice)
     with pytest.raises(ValueError, match="dimension"):
         spec.tree_attention(_on(1, 2, 1, 8, dtype=torch.float16), cache, cache, _on(1, dtype=torch.int32))
+
+
+def test_rope_append_does_not_drop_keys(calls):
+    """A cache that is missing is no reason to rotate q alone and say nothing."""
+    q, kv, cache, lens, table = _on(1, 2, 4, 64), _on(1, 2, 2, 64), _on(1, 2, 8, 64), _on(1, dtype=torch.int32), _on(8, 32)
+    for args in ((kv, kv, table, table, None, None), (kv, kv, table, table, cache, None), (None, kv, table, table, cache, cache),
+                 (kv, None, table, table, cache, cache), (None, None, table, table, None, None)):
+        with pytest.raises(TypeError):
+            spec.rope_append(q, *args, lens)
+    assert not calls
