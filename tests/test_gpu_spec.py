@@ -782,3 +782,32 @@ def test_verify_at_the_smallest_temperatures(temperature):
     want = spec.verify_tree(tokens, z, u, race, par, draft_probs=d, temperature=torch.zeros(4, device="cuda"))
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("T,hq,hkv,hd,window", [(1, 2, 2, 128, 0), (3, 8, 2, 64, 0), (5, 8, 2, 128, 40), (12, 8, 4, 64, 9),
+                                                (11, 8, 2, 80, 0), (30, 4, 2, 64, 0), (13, 8, 2, 128, 0), (64, 6, 2, 64, 70),
+                                                (50, 12, 2, 128, 0)])
+def test_sequences_that_share_one_cache(T, hq, hkv, hd, window, dt):
+    """A cache expanded over the sequences (a stride of zero, which no tensor map describes): one prefix, several trees."""
+    B, n = 3, 500
+    q, kc, vc, lens, par, sk = _attn_case(B, T, hq, hkv, hd, n, True, True, dt)
+    lens.fill_(n)
+    kc, vc = kc[:1].expand(B, -1, -1, -1), vc[:1].expand(B, -1, -1, -1)
+    assert kc.stride(0) == 0
+    node = T // 2
+    trees = [oracle.tree(p, T) for p in par.cpu()]
+    want, smax, vmax = oracle.attention(f64(q), f64(kc), f64(vc), lens.cpu(), par.cpu(), f64(sk), window, hd ** -0.5)
+    out = spec.tree_attention(q, kc, vc, lens, par, sinks=sk, window=window)
+    assert (np.abs(f64(out) - want) <= _attn_tol(dt, smax, vmax, want)).all()
+    own = spec.tree_attention(q, kc.contiguous(), vc.contiguous(), lens, par, sinks=sk, window=window)
+    assert (np.abs(f64(own) - want) <= _attn_tol(dt, smax, vmax, want)).all()
+    vc[0, 0, n + node] = float("nan")            # in the mask's block: its own rows alone
+    out2 = spec.tree_attention(q, kc, vc, lens, par, sinks=sk, window=window)
+    for b in range(B):
+        for t, anc in enumerate(trees[b]):
+            sees = anc is not None and node in anc and (not window or len(anc) - 1 - anc.index(node) < window)
+            got, was = out2[b, t, :hq // hkv], out[b, t, :hq // hkv]
+            assert torch.isnan(got).all() if sees else torch.isfinite(got).all() and (got - was).abs().max() <= 8 * UNIT[dt] * vmax
+    q[0, 0, 0, 1] = float("nan")
+    assert torch.isnan(spec.tree_attention(q, kc, vc, lens, par, sinks=sk, window=window)[0, 0, 0]).all()
