@@ -436,7 +436,9 @@ int ns_rope_append(const ns_rope_append_t* p, ns_stream_t stream);
  * logit per head to the softmax, as neurostream/model/gpt_oss.py:73-87
  * `sink_attention`.  T = 1 is plain decode.  Keys and values of the nodes are in
  * the cache already (ns_rope_append).  out rows of unused nodes, and of nodes
- * that see nothing, are zero; what no node may see is not used, whatever it holds.
+ * that see nothing, are zero; what no node may see is not used, whatever it holds, and
+ * what a node sees counts, whatever it is: a NaN in its query, or in a key or value
+ * that it sees, gives NaN, and so do scores that are all -inf (zero with a sink).
  * q, caches and out have one type: fp32 (products at fp32 precision), fp16 or
  * bf16 (fp32 softmax; probabilities rounded to the type for the product with
  * the values).  head_dim up to 128, a multiple of 8; any number of query heads per kv head.

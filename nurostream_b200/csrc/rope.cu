@@ -11,7 +11,7 @@
 // the heads of one token: one table slice, one division, for all of them.  The heads' elements are read
 // before the token's position is known (length, then depth in the tree, then the table's row: each
 // waits for the one before).  Rows that do not divide into octets on 16 bytes go pair by pair.
-// Measured (device time of a call in a captured graph, 80 heads): one token, fp32, 2.5 us; 528 tree tokens
+// Measured (device time of a call in a captured graph, 80 heads): one token, fp32, 2.7 us; 528 tree tokens
 // of 128 dims, bf16, 7.7 us (2.8 TB/s); 4,098 prompt tokens 41 us (4.1 TB/s, where a copy has 6.5): bound by
 // issue (300 instructions a unit before the addresses ran along) and by blocks that live for one
 // token; blocks that stay and fetch the next token ahead by cp.async were slower (48 us).

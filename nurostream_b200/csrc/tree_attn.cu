@@ -18,13 +18,17 @@
 // Blocks arrive by cp.async in a ring of three stages.  16-bit products are mma.m16n8k16; fp32
 // products split each operand into two tf32 parts and add three mma.m16n8k8 (the product of the two
 // low parts, 2^-22 of the whole, is dropped), and the sum over a block joins the running output in
-// plain fp32 additions.
+// plain fp32 additions.  What the parts cannot hold (infinities, values that round to one) is found and
+// done in plain fp32: such elements make a score NaN, which is then computed again, and every block's
+// values are looked through.
 //
 // Measured (device time of a call in a captured graph, 64 query and 8 kv heads of 64, fp32, 2048 keys,
-// sinks): one token 13.4 us, of which the blocks themselves take 7 and the join 4.5; a tree of 16 nodes
-// (128 rows) 31 us.  The bytes would take 1.3 us: one token is bound by the chain of dependent steps
-// (length, run, block, partial rows, join), the tree by its products, which run at half of what
-// mma.sync has for tf32 (three products each, and the parts are split anew by every warp).
+// sinks): one token 13.3 us, of which the blocks themselves take 7 and the join 4.5; a tree of 16 nodes
+// (128 rows) 31.2 us.  The bytes would take 1.3 us: one token is bound by the chain of dependent steps
+// (length, run, block, partial rows, join), the tree by issue and the latency of its products (tensor pipe
+// 29 % busy, 1.7 instructions a cycle: three products each, and the parts are split anew by every warp).
+// The look through the values costs nothing that shows (31.1 us against 31.6 before it, with the low
+// part's rounding left out at the same time); cvt to tf32 in place of the integer split, 41 us.
 #include <type_traits>
 
 #include "tree.cuh"
@@ -73,8 +77,9 @@ __device__ __forceinline__ float ex2(float x) {
 
 // Probabilities are relative to the running maximum and are divided by their sum last, so a running output is up to
 // as many times a value as there are keys: the largest values would overflow where the result does not.  In the
-// types that have fp32's range all of them are 2^-kShift of that, which is exact (2^24 keys, each up to 2^8:
-// the tensor-core kernel's maximum may lag), and a sink's share is scaled alike.  fp16's values cannot get there.
+// types that have fp32's range all of them are 2^-kTaShift of that, which is exact (2^24 keys, each up to 2^8:
+// the tensor-core kernel's maximum may lag), and a sink's share is scaled alike.  At the other end the last
+// bits of sums below 2^-94 (5e-29) are lost.  fp16's values get to neither.
 template <int DT>
 constexpr float kTaShift = DT == NS_F16 ? 0.f : 32.f;
 static_assert(kTaShift<NS_F32> == 32.f, "0x1p-32f in tree_attn_kernel");

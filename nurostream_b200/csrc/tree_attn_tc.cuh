@@ -14,6 +14,8 @@
 // The maximum that S is taken relative to is let lag: O is rescaled only when a row's maximum has
 // grown by more than 2^8 (probabilities up to 256 are as exact as those up to 1), which after the
 // first blocks is hardly ever, so O stays in tensor memory from block to block.
+// The 32-wide loads and stores of tensor memory are .aligned: a __syncwarp() stands before those that follow code in
+// which lanes may part (rows that exist and do not, loops over a row's ancestors).  It costs nothing that shows.
 // The probabilities that are masked are zero, but zero times a value that is not finite is not: warp 10
 // looks through the value tile of a masked block, zeroes such rows and leaves their bits for the softmax
 // warps, which add them, from the cache, to the rows that see them.
@@ -22,6 +24,7 @@
 //   5 nodes over 131,071 keys, heads of 128        93 us, 5.8 TB/s: the keys' and values' bytes
 //   8 x 64-node trees over up to 16,384 keys, 128  230 us, 940 TFLOP/s; the kernel itself 207
 //   8 x 27-node trees over up to 8,191 keys, 64    69 us; the kernel 56, the join 11
+// (on several GPUs of the kind: 93 to 94, 226 to 236, 69)
 // A slot's period (128 keys) is about 3,400 cycles: 1,900 to 2,000 of softmax (a row per thread: 110 to
 // read the scores, 400 for the maximum, 1,500 for 128 exponentials at 8 cycles a warp each) and then the
 // slot's own products (1,024 cycles at heads of 128, 512 at 64) with the hand-overs around them.  The two
