@@ -18,17 +18,16 @@
 // Blocks arrive by cp.async in a ring of three stages.  16-bit products are mma.m16n8k16; fp32
 // products split each operand into two tf32 parts and add three mma.m16n8k8 (the product of the two
 // low parts, 2^-22 of the whole, is dropped), and the sum over a block joins the running output in
-// plain fp32 additions.  What the parts cannot hold (infinities, values that round to one) is found and
-// done in plain fp32: such elements make a score NaN, which is then computed again, and every block's
-// values are looked through.
+// plain fp32 additions.  What the parts cannot hold (infinities, values that round to one) comes out as
+// NaN: such a score is computed again in plain fp32, and such a row of the output by the second kernel.
 //
 // Measured (device time of a call in a captured graph, 64 query and 8 kv heads of 64, fp32, 2048 keys,
 // sinks): one token 13.3 us, of which the blocks themselves take 7 and the join 4.5; a tree of 16 nodes
 // (128 rows) 31.2 us.  The bytes would take 1.3 us: one token is bound by the chain of dependent steps
 // (length, run, block, partial rows, join), the tree by issue and the latency of its products (tensor pipe
 // 29 % busy, 1.7 instructions a cycle: three products each, and the parts are split anew by every warp).
-// The look through the values costs nothing that shows (31.1 us against 31.6 before it, with the low
-// part's rounding left out at the same time); cvt to tf32 in place of the integer split, 41 us.
+// Looking through every block's values for them at once took 3 to 15 % more for few rows (4 sequences of 8192
+// keys, heads of 128: one token 98 us against 85); cvt to tf32 in place of the integer split 30 %.
 #include <type_traits>
 
 #include "tree.cuh"
@@ -199,7 +198,7 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint
 // x = hi + lo: hi is x rounded to the 11 significant bits of tf32, lo what is left of it, of which the tensor core
 // drops the bits below its own 11 (at most the last bit of x, 2^-23 of it, which rounding would be off by too).
 // NaN stays NaN in one part or both.  Infinities and values that round to one (kTf32Top and above) come out
-// as parts whose products add to NaN: they are looked for and done in plain fp32.
+// as parts whose products add to NaN: what is NaN is done again in plain fp32.
 __device__ __forceinline__ void tf32_split(uint32_t x, uint32_t& hi, uint32_t& lo) {
   hi = (x + 0x1000u) & 0xFFFFE000u;
   lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
@@ -383,10 +382,9 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
       const int nd = key - sp.len;
       return nd < p.T && nd < kTreeMax && (anc[i] >> nd & 1) && (p.window == 0 || dep[i] - S.depth[nd] < p.window);
     };
-    // Values that not every row sees may hold anything, and fp32 products take no infinities: rows of the block that
-    // hold such values are set to zero here and added, for the rows that see them, from the cache below.
-    const bool look = DT == NS_F32 || masked;
-    if (look) {
+    // Values that not every row sees may hold anything: rows of the block that hold what the products cannot take
+    // are set to zero here and added, for the rows that see them, from the cache below.
+    if (masked) {
       scan ^= 1;
       if (tid < 4) S.bad_keys[scan ^ 1][tid] = 0;  // for the next block that looks; its last readers are past the barrier
 #pragma unroll 4
@@ -559,7 +557,7 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
           }
         }
       }
-      if (look) {  // the values left out, for the rows that see them
+      if (masked) {  // the values left out, for the rows that see them
         uint32_t bad = S.bad_keys[scan][kr >> 5] >> (kr & 31);
         if constexpr (SB < 32) bad &= (1u << SB) - 1;
         while (bad) {
@@ -689,6 +687,75 @@ __global__ void __launch_bounds__(kTaThreads, (TaCfg<DT, HD>::kCtas)) tree_attn_
   }
 }
 
+// One fp32 row of the output over all of its keys in plain fp32, by a warp.  For rows that the tensor cores left with NaN in
+// them although their sum is none: infinities, and values that round to one, in blocks without a mask.  A lane
+// takes a key's score, then the warp the dims key after key.  Rare, and slow (2,048 rows of 8,192 keys 24 ms);
+// kept to few registers, since they count for the kernels that call it.  A score of NaN ends it: the row is NaN as it stands.
+template <int HD>
+__device__ __noinline__ void ta_plain_row(const TaArgs& a, int b, int hk, int row) {
+  constexpr int V = HD / 32;
+  const ns_tree_attn_t& p = a.p;
+  const int lane = threadIdx.x & 31, t = row / a.rep, h = hk * a.rep + row % a.rep;
+  const TaSpan sp = ta_span(p, b);
+  bool bad = false;
+  const int32_t* par = p.parents + (int64_t)b * p.T;
+  const uint64_t anc = p.parents ? tree_mask(t, [&](int i) { return par[i]; }, &bad) : chain_mask(t);
+  const int dep = __popcll(anc) - 1;
+  const float* q = static_cast<const float*>(p.q) + b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2];
+  const float* kc = static_cast<const float*>(p.k_cache) + b * p.kc_stride[0] + hk * p.kc_stride[1];
+  const float* vc = static_cast<const float*>(p.v_cache) + b * p.vc_stride[0] + hk * p.vc_stride[1] + lane * V;
+  float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) o[j] = 0.f;
+  for (int c = sp.lo; c < sp.hi; c += 32) {
+    const int key = c + lane, nd = key - sp.len;
+    bool see = key < sp.hi;
+    if (see && nd < 0) see = p.window == 0 || sp.len + dep - key < p.window;
+    else if (see)  // (an ancestor's depth: the ancestors before it)
+      see = nd < kTreeMax && (anc >> nd & 1) && (p.window == 0 || dep - __popcll(anc & ((1ull << nd) - 1)) < p.window);
+    float x = 0.f;
+    if (see) {
+      const float4* k = reinterpret_cast<const float4*>(kc + (int64_t)key * p.kc_stride[2]);
+#pragma unroll 2
+      for (int d = 0; d < p.head_dim / 4; ++d) {
+        const float4 y = k[d];
+        x = fmaf(q[4 * d], y.x, x), x = fmaf(q[4 * d + 1], y.y, x), x = fmaf(q[4 * d + 2], y.z, x), x = fmaf(q[4 * d + 3], y.w, x);
+      }
+    }
+    x = see ? x * p.scale * 1.4426950408889634f : -INFINITY;
+    if (__any_sync(0xffffffffu, x != x)) return;
+    float mn = fmaxf(m, x);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, i));
+    const float ref = mn == -INFINITY ? 0.f : mn, f = ex2(m - ref), e = ex2(x - ref) * 0x1p-32f;
+    m = mn;
+    l = l * f + warp_sum(e);
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] *= f;
+    const uint32_t seen = __ballot_sync(0xffffffffu, see);
+#pragma unroll 1
+    for (int i = 0; i < 32; i += 4) {
+      float v[4][V];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          v[u][j] = (seen >> (i + u) & 1) && lane * V + j < p.head_dim ? vc[(int64_t)(c + i + u) * p.vc_stride[2] + j] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float w = __shfl_sync(0xffffffffu, e, i + u);
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = fmaf(w, v[u][j], o[j]);
+      }
+    }
+  }
+  const float scale = ta_row_scale<NS_F32>(m, l, p.sinks, h);
+  float* out = static_cast<float*>(p.out) + b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2] + lane * V;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (lane * V + j < p.head_dim) out[j] = o[j] * scale;
+}
+
 // Joins the partial rows of items that were cut between runs.  A block takes a few rows of one item; the
 // item's place in the list, and so which runs hold its parts, is worked out once.  WPR = 1: a warp
 // takes whole rows, two or three parts each.  WPR = 8: few rows and many parts, a row's parts are shared
@@ -730,8 +797,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const _
   const int nblk = (sp.hi - sp.lo + BN - 1) / BN;
   const int64_t s = (before * p.n_head_kv + (int64_t)hk * nblk) * a.row_tiles + (int64_t)rt * nblk, e = s + nblk;
   const int i0 = nblk ? (int)(((s + 1) * runs - 1) / total) : 0, i1 = nblk ? (int)((e * runs - 1) / total) : 0;
-  if (nblk && i0 == i1) return;  // one run covered it
-  const int n = i1 - i0 + 1;
+  const bool whole = nblk && i0 == i1;  // one run covered it
+  // (fp32: a row's open blocks may have left NaN in it, see ta_plain_row)
+  if (whole && (DT != NS_F32 || sp.len - sp.lo < BN)) return;
+  const int n = whole ? 0 : i1 - i0 + 1;
 
   auto finish = [&](int r, float mt, float lt, float (&acc)[V]) {  // one row out
     const int row = rt * MR + r, t = row / a.rep, h = hk * a.rep + row % a.rep;
@@ -761,6 +830,28 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const _
       v[0] = x.x, v[1] = x.y;
     }
   };
+
+  if constexpr (DT == NS_F32) {
+    if (whole) {  // what the run wrote, the warp's rows side by side
+      if (WPR > 1 && warp > 0) return;
+      constexpr int R = WPR > 1 ? 1 : kJoinRows;
+      bool odd[R];
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const int row = rt * MR + min(r0 + k * kJoinWarps + warp, n_rows - 1), t = row / a.rep;
+        const float* out = static_cast<const float*>(p.out) + b * p.o_stride[0] + t * p.o_stride[1] +
+                           (hk * a.rep + row % a.rep) * p.o_stride[2];
+        odd[k] = false;
+#pragma unroll
+        for (int j = 0; j < V; ++j) odd[k] |= lane + 32 * j < p.head_dim && out[lane + 32 * j] != out[lane + 32 * j];
+      }
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+        if (__any_sync(0xffffffffu, odd[k]) && r0 + k * kJoinWarps + warp < n_rows)
+          ta_plain_row<HD>(a, b, hk, rt * MR + r0 + k * kJoinWarps + warp);
+      return;
+    }
+  }
 
   if constexpr (WPR == 1) {
     // the warp's rows side by side: their loads are in flight together
@@ -794,7 +885,26 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const _
 #pragma unroll
     for (int k = 0; k < kJoinRows; ++k) {
       const int r = r0 + k * kJoinWarps + warp;
-      if (r < n_rows) finish(r, mt[k], lt[k], acc[k]);
+      if (r >= n_rows) continue;
+      finish(r, mt[k], lt[k], acc[k]);
+    }
+    if constexpr (DT == NS_F32) {
+      bool odd = false;
+#pragma unroll
+      for (int k = 0; k < kJoinRows; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) odd |= acc[k][j] != acc[k][j];
+      if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+        for (int k = 0; k < kJoinRows; ++k) {
+          const int r = r0 + k * kJoinWarps + warp;
+          bool mine = false;
+#pragma unroll
+          for (int j = 0; j < V; ++j) mine |= acc[k][j] != acc[k][j];
+          if (__any_sync(0xffffffffu, mine) && r < n_rows && mt[k] != -INFINITY && lt[k] == lt[k])
+            ta_plain_row<HD>(a, b, hk, rt * MR + r);
+        }
+      }
     }
   } else {
     float mt = -INFINITY, lt = 0.f, acc[V];
@@ -854,6 +964,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_attn_join_kernel(const _
         for (int j = 0; j < V; ++j) acc[j] = fmaf(so[w][lane * V + j], f, acc[j]);
       }
       finish(r0, mt, lt, acc);
+      if constexpr (DT == NS_F32) {
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < V; ++j) odd |= acc[j] != acc[j];
+        if (__any_sync(0xffffffffu, odd) && mt != -INFINITY && lt == lt) ta_plain_row<HD>(a, b, hk, rt * MR + r0);
+      }
     }
   }
   if (lane == 0 && warp == 0 && r0 == 0 && (p.lens[b] < 0 || p.lens[b] > p.max_ctx)) raise_device_error(NS_DEVERR_ROUTE);

@@ -263,7 +263,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     q: (B, T, n_head, hd), rotated; caches (B, n_head_kv, max_ctx, hd) that hold the nodes' own keys and values at
     slots lens[b] + t already (``rope_append``); one float type for all.  hd a multiple of 8 up to 128, T <= MAX_NODES
     (T = 1: plain decode).  sinks: (n_head,) fp32 extra logits of the softmax.  window > 0: only positions above the
-    node's own minus window.  scale: 1 / sqrt(hd) by default.  Returns (B, T, n_head, hd); zero rows for unused nodes.
+    node's own minus window.  scale: 1 / sqrt(hd) by default.  out may not share memory with q.  Returns (B, T, n_head, hd); zero rows for unused nodes.
     """
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
     key = ("attn", _sig(q), _sig(k_cache), _sig(v_cache), _sig(o), _sig(lens), _sig(parents), _sig(sinks), window, scale)

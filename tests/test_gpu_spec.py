@@ -811,3 +811,35 @@ def test_sequences_that_share_one_cache(T, hq, hkv, hd, window, dt):
             assert torch.isnan(got).all() if sees else torch.isfinite(got).all() and (got - was).abs().max() <= 8 * UNIT[dt] * vmax
     q[0, 0, 0, 1] = float("nan")
     assert torch.isnan(spec.tree_attention(q, kc, vc, lens, par, sinks=sk, window=window)[0, 0, 0]).all()
+
+
+@pytest.mark.parametrize("B,T,hq,hkv,hd", [(200, 2, 8, 2, 64), (512, 1, 2, 2, 128), (60, 20, 12, 2, 64), (30, 33, 8, 2, 128)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_fp32_values_of_open_blocks_in_whole_items(B, T, hq, hkv, hd, window):
+    """Many short sequences: one run writes a row whole, with an infinity, the largest value or a NaN among its keys."""
+    n, rep = 300, hq // hkv
+    q, kc, vc, lens, par, sk = _attn_case(B, T, hq, hkv, hd, n, T > 1, True, F32)
+    want, smax, vmax = oracle.attention(f64(q[:12]), f64(kc[:12]), f64(vc[:12]), lens.cpu(), None if par is None else par.cpu(),
+                                        f64(sk), window, hd ** -0.5)
+    base = spec.tree_attention(q, kc, vc, lens, par, sinks=sk, window=window)
+    top = torch.finfo(F32).max
+    cases = {3: float("inf"), 4: top, 6: "nan", 7: float("-inf"), 9: -top}
+    for b, value in cases.items():
+        _put(vc[b, 0, int(lens[b]) - 99 if window else 10, 5], value)   # (seen by every node without a window)
+    out = spec.tree_attention(q, kc, vc, lens, par, sinks=sk, window=window)
+    wide, _, _ = oracle.attention(f64(q[:12]), f64(kc[:12]), f64(vc[:12]), lens.cpu(), None if par is None else par.cpu(),
+                                  f64(sk), window, hd ** -0.5)
+    got = f64(out[:12])
+    for b, value in cases.items():
+        col, ref, plain = got[b, :, :rep, 5].copy(), wide[b, :, :rep, 5], want[b, :, :rep, 5]
+        hit = ref != plain                                             # rows that see the value
+        assert hit.any()
+        if value == "nan":
+            assert np.isnan(col[hit]).all()
+        elif abs(value) == top:
+            assert (np.abs(col - ref) <= _attn_tol(F32, smax, top, ref))[hit].all()
+        else:
+            assert (col[hit] == value).all()
+        got[b, :, :rep, 5][hit] = plain[hit]
+    assert (np.abs(got - want) <= _attn_tol(F32, smax, vmax, want)).all()
+    assert torch.equal(out[12:], base[12:])
