@@ -22,10 +22,10 @@
 // NaN: such a score is computed again in plain fp32, and such a row of the output by the second kernel.
 //
 // Measured (device time of a call in a captured graph, 64 query and 8 kv heads of 64, fp32, 2048 keys,
-// sinks): one token 13.3 us, of which the blocks themselves take 7 and the join 4.5; a tree of 16 nodes
-// (128 rows) 31.2 us.  The bytes would take 1.3 us: one token is bound by the chain of dependent steps
+// sinks): one token 13.4 us, of which the blocks themselves take 7 and the join 4.5; a tree of 16 nodes
+// (128 rows) 31.5 us.  The bytes would take 1.3 us: one token is bound by the chain of dependent steps
 // (length, run, block, partial rows, join), the tree by issue and the latency of its products (tensor pipe
-// 29 % busy, 1.7 instructions a cycle: three products each, and the parts are split anew by every warp).
+// 30 % busy, 1.7 instructions a cycle: three products each, and the parts are split anew by every warp).
 // Looking through every block's values for them at once took 3 to 15 % more for few rows (4 sequences of 8192
 // keys, heads of 128: one token 98 us against 85); cvt to tf32 in place of the integer split 30 %.
 #include <type_traits>

@@ -24,7 +24,7 @@
 //   5 nodes over 131,071 keys, heads of 128        93 us, 5.8 TB/s: the keys' and values' bytes
 //   8 x 64-node trees over up to 16,384 keys, 128  230 us, 940 TFLOP/s; the kernel itself 207
 //   8 x 27-node trees over up to 8,191 keys, 64    69 us; the kernel 56, the join 11
-// (on several GPUs of the kind: 93 to 94, 226 to 236, 69)
+// (on several GPUs of the kind: 92 to 94, 226 to 236, 69)
 // A slot's period (128 keys) is about 3,400 cycles: 1,900 to 2,000 of softmax (a row per thread: 110 to
 // read the scores, 400 for the maximum, 1,500 for 128 exponentials at 8 cycles a warp each) and then the
 // slot's own products (1,024 cycles at heads of 128, 512 at 64) with the hand-overs around them.  The two
