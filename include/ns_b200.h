@@ -443,6 +443,7 @@ int ns_rope_append(const ns_rope_append_t* p, ns_stream_t stream);
  * bf16 (fp32 softmax; probabilities rounded to the type for the product with
  * the values).  head_dim up to 128, a multiple of 8; any number of query heads per kv head.
  * Caches: 16-byte aligned, their strides multiples of 16 bytes.
+ * out must not overlap q.
  * Workspace: ns_tree_attn_workspace_bytes, 256-byte aligned, no initialisation.
  */
 typedef struct ns_tree_attn {
